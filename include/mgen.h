@@ -412,6 +412,41 @@ int mgen_attn_decode_prep(const void* qkv, long ld_in, const float* wq, const fl
                           void* out, long ld_o, float* workspace, int B, int H, int KVH, int D, int max_len, int nsplit,
                           float scale, mgen_stream_t stream);
 
+/* ---- KV cache in 4 or 8 bits -------------------------------------------------------------------------------------
+ * The cache of mgen_kv_append in blocks of 32 consecutive elements of a head: one scale byte e and 32 codes, value =
+ * code * 2^(e - 127). bits = 8: e4m3 codes, a byte each; bits = 4: e2m1 codes, the even element in the low half of its
+ * byte. codes [B][KVH][max_len][D * bits / 8] (16-byte aligned), scales [B][KVH][max_len][D / 32], D = 64 or 128. e is the
+ * smallest exponent (1 .. 246 for e4m3, 1 .. 252 for e2m1) at which the block's largest magnitude is at most 464 (e4m3) or
+ * 7 (e2m1) times 2^(e - 127); codes are the nearest, ties to even. A block with an infinity or a NaN has e = 255, codes of
+ * zero, and reads as NaN.
+ * mgen_kv_append_mx quantises n_new tokens per stream from token-major rows (k_src/v_src [B*n_new][ld] bf16, heads at h*D)
+ * into slots pos0[b] .. pos0[b]+n_new-1; mgen_kv_read_mx is the inverse (bf16 values into k_dst/v_dst). Slots outside
+ * [0, max_len) are neither written nor read (the destination row stays as it was). */
+int mgen_kv_append_mx(const void* k_src, const void* v_src, long ld_k, long ld_v, void* k_codes, void* k_scales,
+                      void* v_codes, void* v_scales, const int* pos0, int B, int n_new, int KVH, int D, int max_len,
+                      int bits, mgen_stream_t stream);
+int mgen_kv_read_mx(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                    const int* pos0, void* k_dst, void* v_dst, long ld_k, long ld_v, int B, int n, int KVH, int D,
+                    int max_len, int bits, mgen_stream_t stream);
+/* mgen_attn_decode over that cache (TF models/qwen3/modeling_qwen3.py:259-279 with q_len = 1): softmax statistics, weights
+ * and sums in fp32. kv_len[b] = keys of stream b: 0 (or less) gives an output row of zeros, more than max_len counts as
+ * max_len. nsplit (1 .. 64) workgroups share a stream's keys; mgen_attn_decode_mx_splits suggests a count for calls whose
+ * longest stream has `longest` keys; nsplit > 1 needs mgen_attn_decode_workspace(B, H, D, nsplit) floats. */
+int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest);
+int mgen_attn_decode_mx(const void* q, long ld_q, const void* k_codes, const void* k_scales, const void* v_codes,
+                        const void* v_scales, const int* kv_len, void* out, long ld_o, float* workspace, int B, int H,
+                        int KVH, int D, int max_len, int bits, int nsplit, float scale, mgen_stream_t stream);
+/* mgen_attn_decode_prep over that cache: the new token's rows come from the raw projection output qkv [B][ld_in]; its key
+ * and value are quantised, written to slot pos[b] and attended as they will be read later (the bits of
+ * mgen_decode_qkv_prep's rows through mgen_kv_append_mx, then mgen_attn_decode_mx). cos_sin has npos rows. kv_len[b] must
+ * be pos[b] + 1; a stream for which it is not, or whose pos[b] is outside [0, min(max_len, npos)), gets an output row of
+ * zeros and nothing of its cache is written. */
+int mgen_attn_decode_prep_mx(const void* qkv, long ld_in, const float* wq, const float* wk, const float* cos_sin,
+                             int npos, const int* pos, float eps, int interleaved, void* k_codes, void* k_scales,
+                             void* v_codes, void* v_scales, const int* kv_len, void* out, long ld_o, float* workspace,
+                             int B, int H, int KVH, int D, int max_len, int bits, int nsplit, float scale,
+                             mgen_stream_t stream);
+
 /* ---- sampler -------------------------------------------------------------------------------------------------
  * GenerationMixin._sample token selection (TF generation/utils.py:2894-2925) with the warpers
  * TF generation/logits_process.py:301-303 (temperature), :590-595 (top-k), :527-539 (top-p), in that order.

@@ -92,6 +92,11 @@ SIGNATURES = {
     "mgen_decode_layer": [P] * 22 + [I] * 8 + [F, I, P],
     "mgen_decode_qkv_prep": [P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, F, I, P],
     "mgen_attn_decode_prep": [P, L, P, P, P, P, F, I, P, P, P, P, L, P, I, I, I, I, I, I, F, P],
+    "mgen_kv_append_mx": [P, P, L, L, P, P, P, P, P, I, I, I, I, I, I, P],
+    "mgen_kv_read_mx": [P, P, P, P, P, P, P, L, L, I, I, I, I, I, I, P],
+    "mgen_attn_decode_mx_splits": [I, I, I, I, I],
+    "mgen_attn_decode_mx": [P, L, P, P, P, P, P, P, L, P, I, I, I, I, I, I, I, F, P],
+    "mgen_attn_decode_prep_mx": [P, L, P, P, P, I, P, F, I, P, P, P, P, P, P, L, P, I, I, I, I, I, I, I, F, P],
     "mgen_sample_rows": [P, L, I, I, I, I, F, I, F, P, L, U64, U64, I, P, P, L, P],
     "mgen_sample": [P, L, I, I, I, I, F, I, F, P, L, U64, U64, P, P, L, P],
     "mgen_sample_step": [P, L, I, I, I, I, F, I, F, P, L, U64, U64, I, P, P, L, P, P, L, L, P],

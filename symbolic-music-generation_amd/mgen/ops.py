@@ -603,6 +603,133 @@ def attn_decode_workspace(B, H, D, nsplit):
     return lib().mgen_attn_decode_workspace(B, H, D, nsplit)
 
 
+MX_BITS = {"mxfp4": 4, "mxfp8": 8}
+
+
+class MXKV:
+    """One layer's keys and values in blocks of 32 elements with a shared power-of-two scale (include/mgen.h, "KV cache in
+    4 or 8 bits"): codes k, v uint8 [B, KVH, max_len, D or D/2], scales k_scale, v_scale uint8 [B, KVH, max_len, D/32]."""
+
+    __slots__ = ("k", "k_scale", "v", "v_scale", "B", "KVH", "max_len", "D", "bits", "fmt", "device", "ptrs")
+
+    def __init__(self, k, k_scale, v, v_scale):
+        for t in (k, k_scale, v, v_scale):
+            if t.dtype != torch.uint8 or t.dim() != 4 or not t.is_contiguous():
+                raise ValueError("a quantised cache consists of contiguous 4-dimensional uint8 tensors")
+        if v.shape != k.shape or v_scale.shape != k_scale.shape or k_scale.shape[:3] != k.shape[:3]:
+            raise ValueError(f"keys and values, codes and scales must agree in shape: codes {tuple(k.shape)} and "
+                             f"{tuple(v.shape)}, scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
+        self.B, self.KVH, self.max_len = k.shape[:3]
+        self.D = 32 * k_scale.shape[3]
+        self.bits = {self.D // 2: 4, self.D: 8}.get(k.shape[3])
+        if self.D not in (64, 128) or self.bits is None:
+            raise ValueError(f"head_dim 64 or 128 with codes of 4 or 8 bits: got codes of {k.shape[3]} bytes and "
+                             f"{k_scale.shape[3]} scales a row")
+        if len({t.device for t in (k, k_scale, v, v_scale)}) != 1:
+            raise ValueError("the parts of a quantised cache must be on one device")
+        if k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise ValueError("the codes of a quantised cache must be 16-byte aligned")
+        _need_gpu(k)
+        self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
+        self.fmt = "mxfp4" if self.bits == 4 else "mxfp8"
+        self.device = k.device
+        self.ptrs = (k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr())
+
+    @classmethod
+    def empty(cls, B, KVH, max_len, D, fmt, device):
+        if fmt not in MX_BITS:
+            raise ValueError(f"cache type {fmt!r}: one of {sorted(MX_BITS)}")
+        t = [torch.empty(B, KVH, max_len, w, dtype=torch.uint8, device=device)
+             for w in (D * MX_BITS[fmt] // 8, D // 32) * 2]
+        return cls(*t)
+
+    def streams(self, b0, b1):
+        """Streams [b0, b1) (views)."""
+        return MXKV(self.k[b0:b1], self.k_scale[b0:b1], self.v[b0:b1], self.v_scale[b0:b1])
+
+    def _check(self, B, **per_stream):
+        if not 0 < B <= self.B:
+            raise ValueError(f"{B} streams, the cache holds {self.B}")
+        if self.device.index != torch.cuda.current_device():
+            raise RuntimeError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+        for name, t in per_stream.items():
+            if t.dtype != torch.int32 or t.numel() < B or not t.is_contiguous() or t.device != self.device:
+                raise ValueError(f"{name} must be a contiguous int32 tensor of {B} entries on {self.device}")
+
+    def _rows(self, x, name, n, ld, width):
+        """Address of [n][ld] bf16 rows of which `width` elements are used: a raw device pointer (int) as it is, a
+        2-dimensional tensor after checks."""
+        if ld < width:
+            raise ValueError(f"{name}: a row stride of {ld} for rows of {width} elements")
+        if isinstance(x, int):
+            return x
+        if x.dtype != torch.bfloat16 or x.device != self.device or x.dim() != 2 or x.stride(1) != 1:
+            raise ValueError(f"{name} must be a 2-dimensional bfloat16 tensor on {self.device} with unit element stride")
+        if x.shape[0] < n or x.shape[1] < width or (n > 1 and x.stride(0) != ld):
+            raise ValueError(f"{name}: {n} rows of {width} elements with stride {ld} from a tensor of shape "
+                             f"{tuple(x.shape)} with stride {x.stride(0)}")
+        return x.data_ptr()
+
+
+def kv_append_mx(k_src, v_src, ld_k, ld_v, kv, pos0, B, n_new):
+    """kv_append into a quantised cache: rows k_src/v_src [B*n_new][ld] bf16 (tensors or raw device pointers) into slots
+    pos0[b] .. pos0[b] + n_new - 1 of stream b; slots outside the cache are skipped."""
+    kv._check(B, pos0=pos0)
+    w = kv.KVH * kv.D
+    call("mgen_kv_append_mx", kv._rows(k_src, "k_src", B * n_new, ld_k, w), kv._rows(v_src, "v_src", B * n_new, ld_v, w),
+         ld_k, ld_v, *kv.ptrs, pos0.data_ptr(), B, n_new, kv.KVH, kv.D, kv.max_len, kv.bits, _stream())
+
+
+def kv_read_mx(kv, pos0, k_dst, v_dst, ld_k, ld_v, B, n):
+    """The inverse of kv_append_mx: the values of slots pos0[b] .. pos0[b] + n - 1 into rows k_dst/v_dst [B*n][ld] bf16;
+    rows whose slot is outside the cache stay as they were."""
+    kv._check(B, pos0=pos0)
+    w = kv.KVH * kv.D
+    call("mgen_kv_read_mx", *kv.ptrs, pos0.data_ptr(), kv._rows(k_dst, "k_dst", B * n, ld_k, w),
+         kv._rows(v_dst, "v_dst", B * n, ld_v, w), ld_k, ld_v, B, n, kv.KVH, kv.D, kv.max_len, kv.bits, _stream())
+
+
+def attn_decode_mx_splits(B, H, KVH, D, longest):
+    """Key splits for attention over a quantised cache whose longest stream has `longest` keys."""
+    from ._lib import lib
+    return lib().mgen_attn_decode_mx_splits(B, H, KVH, D, longest)
+
+
+def _mx_workspace(workspace, B, H, D, nsplit):
+    if nsplit > 1:
+        if workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous() or not workspace.is_cuda:
+            raise ValueError("nsplit > 1 needs a contiguous fp32 workspace on the GPU")
+        if workspace.numel() < attn_decode_workspace(B, H, D, nsplit):
+            raise ValueError(f"a workspace of {workspace.numel()} floats, attn_decode_workspace asks for "
+                             f"{attn_decode_workspace(B, H, D, nsplit)}")
+    return _p(workspace)
+
+
+def attn_decode_mx(q, ld_q, kv, kv_len, out, ld_o, workspace, B, H, nsplit, scale):
+    """attn_decode over a quantised cache (an MXKV). q/out: rows [B][ld] bf16 (tensors or raw device pointers); a stream
+    with kv_len[b] = 0 gets zeros, kv_len[b] beyond the cache counts as the cache's length."""
+    kv._check(B, kv_len=kv_len)
+    D = kv.D
+    call("mgen_attn_decode_mx", kv._rows(q, "q", B, ld_q, H * D), ld_q, *kv.ptrs, kv_len.data_ptr(),
+         kv._rows(out, "out", B, ld_o, H * D), ld_o, _mx_workspace(workspace, B, H, D, nsplit), B, H, kv.KVH, D,
+         kv.max_len, kv.bits, nsplit, scale, _stream())
+
+
+def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_len, out, ld_o, workspace, B, H, nsplit,
+                        scale):
+    """attn_decode_prep over a quantised cache (an MXKV): q, new key and value from the raw projection rows, the new row
+    quantised into slot pos[b] and attended. A stream whose pos[b] is no row of the cache or of the rotary table cs, or
+    whose kv_len[b] is not pos[b] + 1, gets zeros and is not written."""
+    kv._check(B, pos=pos, kv_len=kv_len)
+    D = kv.D
+    for t, n, name in ((wq, D, "wq"), (wk, D, "wk"), (cs, D, "cs")):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.device != kv.device or t.numel() < n):
+            raise ValueError(f"{name} must be a contiguous fp32 tensor on {kv.device}")
+    call("mgen_attn_decode_prep_mx", kv._rows(qkv, "qkv", B, ld_in, (H + 2 * kv.KVH) * D), ld_in, _p(wq), _p(wk), _p(cs),
+         cs.numel() // D, _p(pos), eps, int(interleaved), *kv.ptrs, _p(kv_len), kv._rows(out, "out", B, ld_o, H * D),
+         ld_o, _mx_workspace(workspace, B, H, D, nsplit), B, H, kv.KVH, D, kv.max_len, kv.bits, nsplit, scale, _stream())
+
+
 def sample(logits, V, out, do_sample=False, temperature=1.0, top_k=0, top_p=1.0, noise=None, seed=0, offset=0,
            out2=None, out2_stride=0, row0=0, step=None, unfinished=None, eos_id=0, pad_id=0):
     """logits [B, ld] (bf16 or fp32) -> out [B] int64; out2 = raw pointer of an optional strided second destination.

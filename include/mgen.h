@@ -447,6 +447,14 @@ int mgen_attn_decode_prep_mx(const void* qkv, long ld_in, const float* wq, const
                              int B, int H, int KVH, int D, int max_len, int bits, int nsplit, float scale,
                              mgen_stream_t stream);
 
+/* mgen_decode_layer over that cache (mgen_decode_layer_fits holds for both). */
+int mgen_decode_layer_mx(void* x, const float* h_in, float* h_mid, float* h_out, void* qkv, void* att, void* gu,
+                         float* slabs, float* attn_workspace, const void* w_qkv, const float* w_qn, const float* w_kn,
+                         const void* w_o, const float* w_ln2, const void* w_gu, const void* w_down, const float* w_next,
+                         const float* cos_sin, int npos, const int* pos, const int* kv_len, void* k_codes,
+                         void* k_scales, void* v_codes, void* v_scales, int B, int d, int H, int KVH, int D, int I,
+                         int max_len, int bits, int nsplit, float eps, int interleaved, mgen_stream_t stream);
+
 /* ---- sampler -------------------------------------------------------------------------------------------------
  * GenerationMixin._sample token selection (TF generation/utils.py:2894-2925) with the warpers
  * TF generation/logits_process.py:301-303 (temperature), :590-595 (top-k), :527-539 (top-p), in that order.

@@ -16,6 +16,11 @@ extern "C" int mgen_attn_decode_prep(const void* qkv, long ld_in, const float* w
                                      const float* cos_sin, const int* pos, float eps, int interleaved, void* k_cache,
                                      void* v_cache, const int* kv_len, void* out, long ld_o, float* workspace, int B,
                                      int H, int KVH, int D, int max_len, int nsplit, float scale, hipStream_t stream);
+extern "C" int mgen_attn_decode_prep_mx(const void* qkv, long ld_in, const float* wq, const float* wk,
+                                        const float* cos_sin, int npos, const int* pos, float eps, int interleaved,
+                                        void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int* kv_len,
+                                        void* out, long ld_o, float* workspace, int B, int H, int KVH, int D,
+                                        int max_len, int bits, int nsplit, float scale, hipStream_t stream);
 extern "C" int mgen_slab_resid_rmsnorm(const float* slabs, int nslabs, long slab_stride, const float* resid,
                                        float* h_out, const float* w, void* y, long T, int d, float eps, int round_bf16,
                                        hipStream_t stream);
@@ -37,30 +42,66 @@ extern "C" int mgen_decode_layer_fits(int B, int d, int H, int KVH, int D, int I
 // weights: w_qkv [(H+2KVH)D][d], w_o [d][HD], w_gu [2I][d], w_down [d][I] bf16; gains fp32: w_qn, w_kn [D] (both may be
 // null), w_ln2 [d] (post-attention norm), w_next [d] (the norm that follows the layer)
 // pos[b] = position of the new token, kv_len[b] = pos[b] + 1; caches [B][KVH][max_len][D] bf16
-extern "C" int mgen_decode_layer(void* x, const float* h_in, float* h_mid, float* h_out, void* qkv, void* att, void* gu,
-                                 float* slabs, float* attn_workspace, const void* w_qkv, const float* w_qn,
-                                 const float* w_kn, const void* w_o, const float* w_ln2, const void* w_gu,
-                                 const void* w_down, const float* w_next, const float* cos_sin, const int* pos,
-                                 const int* kv_len, void* k_cache, void* v_cache, int B, int d, int H, int KVH, int D,
-                                 int I, int max_len, int nsplit, float eps, int interleaved, hipStream_t stream) {
+namespace {
+
+// the launches of a layer; attend(scale) issues the attention over the cache (qkv -> att)
+template <typename Attend>
+int decode_layer(const char* what, void* x, const float* h_in, float* h_mid, float* h_out, void* qkv, void* att, void* gu,
+                 float* slabs, const void* w_qkv, const void* w_o, const float* w_ln2, const void* w_gu,
+                 const void* w_down, const float* w_next, int B, int d, int H, int KVH, int D, int I, float eps,
+                 hipStream_t stream, Attend attend) {
     MGEN_REQUIRE(x && h_in && h_mid && h_out && qkv && att && gu && slabs && w_qkv && w_o && w_ln2 && w_gu && w_down &&
-                     w_next && cos_sin && pos && kv_len && k_cache && v_cache,
-                 "mgen_decode_layer: null pointer");
-    MGEN_REQUIRE(mgen_decode_layer_fits(B, d, H, KVH, D, I), "mgen_decode_layer: shapes not taken (B=%d d=%d H=%d KVH=%d "
-                 "D=%d I=%d): see mgen_decode_layer_fits", B, d, H, KVH, D, I);
+                     w_next,
+                 "%s: null pointer", what);
+    MGEN_REQUIRE(mgen_decode_layer_fits(B, d, H, KVH, D, I), "%s: shapes not taken (B=%d d=%d H=%d KVH=%d "
+                 "D=%d I=%d): see mgen_decode_layer_fits", what, B, d, H, KVH, D, I);
     const int NQ = (H + 2 * KVH) * D, HD = H * D;
     const long bd = (long)B * d;
-    const float scale = 1.0f / sqrtf((float)D);
     if (int e = mgen_gemm_bf16_skinny(x, w_qkv, qkv, B, NQ, d, d, d, NQ, 0, 0, 0, stream)) return e;
-    if (int e = mgen_attn_decode_prep(qkv, NQ, w_qn, w_kn, cos_sin, pos, eps, interleaved, k_cache, v_cache, kv_len, att,
-                                      HD, attn_workspace, B, H, KVH, D, max_len, nsplit, scale, stream))
-        return e;
+    if (int e = attend(1.0f / sqrtf((float)D))) return e;
     const int ns_o = mgen_gemm_skinny_slabs(B, d, HD), ns_d = mgen_gemm_skinny_slabs(B, d, I);
     if (int e = mgen_gemm_bf16_skinny(att, w_o, slabs, B, d, HD, HD, HD, d, ns_o, bd, 0, stream)) return e;
     if (int e = mgen_slab_resid_rmsnorm(slabs, ns_o, bd, h_in, h_mid, w_ln2, x, B, d, eps, 1, stream)) return e;
     if (int e = mgen_gemm_bf16_skinny(x, w_gu, gu, B, 2 * I, d, d, d, 2 * I, 0, 0, 0, stream)) return e;
     if (int e = mgen_gemm_bf16_skinny(gu, w_down, slabs, B, d, I, 2L * I, I, d, ns_d, bd, 1, stream)) return e;
     return mgen_slab_resid_rmsnorm(slabs, ns_d, bd, h_mid, h_out, w_next, x, B, d, eps, 1, stream);
+}
+
+}  // namespace
+
+extern "C" int mgen_decode_layer(void* x, const float* h_in, float* h_mid, float* h_out, void* qkv, void* att, void* gu,
+                                 float* slabs, float* attn_workspace, const void* w_qkv, const float* w_qn,
+                                 const float* w_kn, const void* w_o, const float* w_ln2, const void* w_gu,
+                                 const void* w_down, const float* w_next, const float* cos_sin, const int* pos,
+                                 const int* kv_len, void* k_cache, void* v_cache, int B, int d, int H, int KVH, int D,
+                                 int I, int max_len, int nsplit, float eps, int interleaved, hipStream_t stream) {
+    MGEN_REQUIRE(cos_sin && pos && kv_len && k_cache && v_cache, "mgen_decode_layer: null pointer");
+    return decode_layer("mgen_decode_layer", x, h_in, h_mid, h_out, qkv, att, gu, slabs, w_qkv, w_o, w_ln2, w_gu, w_down,
+                        w_next, B, d, H, KVH, D, I, eps, stream, [&](float scale) {
+                            return mgen_attn_decode_prep(qkv, (H + 2 * KVH) * D, w_qn, w_kn, cos_sin, pos, eps,
+                                                         interleaved, k_cache, v_cache, kv_len, att, H * D,
+                                                         attn_workspace, B, H, KVH, D, max_len, nsplit, scale, stream);
+                        });
+}
+
+// The same layer over a cache in 4 or 8 bits (mgen_attn_decode_prep_mx): codes [B][KVH][max_len][D * bits / 8], scales
+// [B][KVH][max_len][D / 32]; cos_sin has npos rows
+extern "C" int mgen_decode_layer_mx(void* x, const float* h_in, float* h_mid, float* h_out, void* qkv, void* att,
+                                    void* gu, float* slabs, float* attn_workspace, const void* w_qkv, const float* w_qn,
+                                    const float* w_kn, const void* w_o, const float* w_ln2, const void* w_gu,
+                                    const void* w_down, const float* w_next, const float* cos_sin, int npos,
+                                    const int* pos, const int* kv_len, void* k_codes, void* k_scales, void* v_codes,
+                                    void* v_scales, int B, int d, int H, int KVH, int D, int I, int max_len, int bits,
+                                    int nsplit, float eps, int interleaved, hipStream_t stream) {
+    MGEN_REQUIRE(cos_sin && pos && kv_len && k_codes && k_scales && v_codes && v_scales,
+                 "mgen_decode_layer_mx: null pointer");
+    return decode_layer("mgen_decode_layer_mx", x, h_in, h_mid, h_out, qkv, att, gu, slabs, w_qkv, w_o, w_ln2, w_gu,
+                        w_down, w_next, B, d, H, KVH, D, I, eps, stream, [&](float scale) {
+                            return mgen_attn_decode_prep_mx(qkv, (H + 2 * KVH) * D, w_qn, w_kn, cos_sin, npos, pos, eps,
+                                                            interleaved, k_codes, k_scales, v_codes, v_scales, kv_len,
+                                                            att, H * D, attn_workspace, B, H, KVH, D, max_len, bits,
+                                                            nsplit, scale, stream);
+                        });
 }
 
 namespace {

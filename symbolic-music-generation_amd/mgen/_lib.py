@@ -97,6 +97,7 @@ SIGNATURES = {
     "mgen_attn_decode_mx_splits": [I, I, I, I, I],
     "mgen_attn_decode_mx": [P, L, P, P, P, P, P, P, L, P, I, I, I, I, I, I, I, F, P],
     "mgen_attn_decode_prep_mx": [P, L, P, P, P, I, P, F, I, P, P, P, P, P, P, L, P, I, I, I, I, I, I, I, F, P],
+    "mgen_decode_layer_mx": [P] * 18 + [I] + [P] * 6 + [I] * 9 + [F, I, P],
     "mgen_sample_rows": [P, L, I, I, I, I, F, I, F, P, L, U64, U64, I, P, P, L, P],
     "mgen_sample": [P, L, I, I, I, I, F, I, F, P, L, U64, U64, P, P, L, P],
     "mgen_sample_step": [P, L, I, I, I, I, F, I, F, P, L, U64, U64, I, P, P, L, P, P, L, L, P],

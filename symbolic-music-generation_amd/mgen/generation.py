@@ -26,6 +26,9 @@ from . import ops
 
 
 class KVCache:
+    """bf16 keys and values of every layer, [B, KVH, max_len, D] each."""
+    fmt = "bf16"
+
     def __init__(self, cfg, batch: int, max_len: int, device):
         self.max_len = max_len
         shape = (batch, cfg.num_key_value_heads, max_len, cfg.head_dim)
@@ -33,8 +36,23 @@ class KVCache:
         self.v = [torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(cfg.num_hidden_layers)]
         self.zero_pos = torch.zeros(batch, dtype=torch.int32, device=device)
 
+    @property
+    def batch(self):
+        return self.k[0].shape[0]
+
+    @property
+    def device(self):
+        return self.k[0].device
+
+    def tensors(self):
+        return self.k + self.v
+
     def bytes_per_token(self):
         return 2 * len(self.k) * self.k[0].shape[1] * self.k[0].shape[3] * 2
+
+    def part(self, b0: int, b1: int):
+        """The cache of streams [b0, b1) (views: a stream's rows are contiguous)."""
+        return _CachePart(self, b0, b1)
 
     def first_streams(self, batch: int):
         """The cache of the first `batch` streams (views; the row capacity, i.e. the pitch between heads, stays)."""
@@ -42,8 +60,22 @@ class KVCache:
             return self
         return _CachePart(self, 0, batch)
 
+    def append(self, l, k_src, v_src, ld_k, ld_v, pos0, B, n):
+        """n tokens per stream into layer l, from position pos0[b] on (raw pointers of token-major rows)."""
+        _, KVH, _, D = self.k[l].shape
+        ops.kv_append(k_src, v_src, ld_k, ld_v, self.k[l], self.v[l], pos0, B, n, KVH, D, self.max_len)
 
-class _CachePart:
+    def attend(self, l, q, ld_q, kv_len, out, ld_o, ws, B, H, nsplit, scale):
+        _, KVH, _, D = self.k[l].shape
+        ops.attn_decode(q, ld_q, self.k[l], self.v[l], kv_len, out, ld_o, ws, B, H, KVH, D, self.max_len, nsplit, scale)
+
+    def attend_prep(self, l, qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv_len, out, ld_o, ws, B, H, nsplit, scale):
+        _, KVH, _, D = self.k[l].shape
+        ops.attn_decode_prep(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, self.k[l], self.v[l], kv_len, out, ld_o, ws,
+                             B, H, KVH, D, self.max_len, nsplit, scale)
+
+
+class _CachePart(KVCache):
     """Streams [b0, b1) of a KVCache (views: a stream's rows are contiguous)."""
 
     def __init__(self, cache: KVCache, b0: int, b1: int):
@@ -53,12 +85,69 @@ class _CachePart:
         self.zero_pos = cache.zero_pos[b0:b1]
 
 
+class MXKVCache:
+    """Keys and values of every layer in blocks of 32 elements with a shared power-of-two scale: "mxfp8" (e4m3 codes, 8.25
+    bits an element) or "mxfp4" (e2m1 codes, 4.25 bits). The interface of KVCache; kv[l] is layer l's ops.MXKV."""
+
+    def __init__(self, cfg, batch: int, max_len: int, device, fmt: str):
+        self._set([ops.MXKV.empty(batch, cfg.num_key_value_heads, max_len, cfg.head_dim, fmt, device)
+                   for _ in range(cfg.num_hidden_layers)], torch.zeros(batch, dtype=torch.int32, device=device))
+
+    def _set(self, kv, zero_pos):
+        self.kv, self.zero_pos = kv, zero_pos
+        self.fmt, self.batch, self.max_len, self.device = kv[0].fmt, kv[0].B, kv[0].max_len, kv[0].device
+
+    def tensors(self):
+        return [t for kv in self.kv for t in (kv.k, kv.k_scale, kv.v, kv.v_scale)]
+
+    def bytes_per_token(self):
+        return sum(t.numel() for t in self.tensors()) // (self.batch * self.max_len)
+
+    def part(self, b0: int, b1: int):
+        c = object.__new__(MXKVCache)
+        c._set([kv.streams(b0, b1) for kv in self.kv], self.zero_pos[b0:b1])
+        return c
+
+    def first_streams(self, batch: int):
+        return self if batch == self.batch else self.part(0, batch)
+
+    def append(self, l, k_src, v_src, ld_k, ld_v, pos0, B, n):
+        ops.kv_append_mx(k_src, v_src, ld_k, ld_v, self.kv[l], pos0, B, n)
+
+    def attend(self, l, q, ld_q, kv_len, out, ld_o, ws, B, H, nsplit, scale):
+        ops.attn_decode_mx(q, ld_q, self.kv[l], kv_len, out, ld_o, ws, B, H, nsplit, scale)
+
+    def attend_prep(self, l, qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv_len, out, ld_o, ws, B, H, nsplit, scale):
+        ops.attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, self.kv[l], kv_len, out, ld_o, ws, B, H,
+                                nsplit, scale)
+
+    def read(self, l: int, pos0: torch.Tensor, n: int):
+        """The values of n slots per stream of layer l from slot pos0[b] on: (k, v), bf16 [B, n, KVH, D] (zeros where a slot
+        lies outside the cache)."""
+        kv = self.kv[l]
+        w = kv.KVH * kv.D
+        k = torch.zeros(self.batch * n, w, dtype=torch.bfloat16, device=self.device)
+        v = torch.zeros_like(k)
+        ops.kv_read_mx(kv, pos0, k, v, w, w, self.batch, n)
+        shape = (self.batch, n, kv.KVH, kv.D)
+        return k.view(shape), v.view(shape)
+
+
+def make_kv_cache(cfg, batch: int, max_len: int, device, fmt: str = "bf16"):
+    """A KV cache of `fmt`: "bf16", "mxfp8" or "mxfp4"."""
+    if fmt == "bf16":
+        return KVCache(cfg, batch, max_len, device)
+    if fmt not in ops.MX_BITS:
+        raise ValueError(f"kv_cache={fmt!r}: one of 'bf16', 'mxfp8', 'mxfp4'")
+    return MXKVCache(cfg, batch, max_len, device, fmt)
+
+
 class _Part:
     """One independently decoded part of the batch: streams [b0, b1), its buffers, cache views and HIP stream."""
 
     def __init__(self, cfg, cache, b0, b1, nxt, ws_floats, dev, stream):
         self.b0, self.b1, self.stream = b0, b1, stream
-        self.cache = _CachePart(cache, b0, b1)
+        self.cache = cache.part(b0, b1)
         self.buf = _DecodeBuffers(cfg, b1 - b0, dev, nxt[b0:b1])
         self.ws = torch.empty(max(ws_floats, 1), dtype=torch.float32, device=dev)
 
@@ -114,22 +203,25 @@ class _DecodeBuffers:
 class GenerationMixin:
     """Mixed into MidiLM."""
 
-    def reserve_kv_cache(self, batch: int, max_len: int):
+    def reserve_kv_cache(self, batch: int, max_len: int, kv_cache: str = "bf16"):
         """Serving: allocate the KV cache for `batch` streams of up to `max_len` tokens once and write to all of it, so
         that generate() calls that fit (batch and total length not larger) neither allocate nor take the first-touch
         page faults of fresh device memory (about 170 ms for the 60 GB of 256 streams x 4096 tokens of the default
-        decoder) inside their first step. Held until release_kv_cache()."""
+        decoder) inside their first step. kv_cache: the type of the calls it is for (generate()'s argument). Held until
+        release_kv_cache()."""
         dev = self.flat_shadow.device
-        cache = KVCache(self.cfg, batch, max_len, dev)
-        for t in cache.k + cache.v:
+        cache = make_kv_cache(self.cfg, batch, max_len, dev, kv_cache)
+        for t in cache.tensors():
             t.zero_()
         self._kv_reserved = cache
 
     def release_kv_cache(self):
         self._kv_reserved = None
 
-    def _decode_split(self, B, length):
+    def _decode_split(self, B, length, fmt="bf16"):
         cfg = self.cfg
+        if fmt != "bf16":
+            return ops.attn_decode_mx_splits(B, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, length)
         blocks = B * cfg.num_attention_heads
         want = max(1, 1024 // max(blocks, 1))
         return max(1, min(64, want, (length + 255) // 256))
@@ -160,7 +252,8 @@ class GenerationMixin:
         if _LAYER_IN_ONE_CALL and buf.sk_qkv and buf.sk_gu and buf.sk_o and buf.sk_down and not self._ln:
             # every launch of the layer issued by one library call (the pointer arguments are collected once per
             # layer and buffer set: only the position, the split count and the stream change from step to step)
-            key = (l, cache.k[l].data_ptr())
+            mx = cache.fmt != "bf16"
+            key = (l, cache.kv[l].ptrs[0] if mx else cache.k[l].data_ptr())
             fixed = buf.layer_args.get(key)
             nxt = buf.h2 if h is buf.h0 else buf.h0
             if fixed is None:
@@ -169,9 +262,14 @@ class GenerationMixin:
                     [t_.data_ptr() for t_ in (buf.x, h, buf.h1, nxt, buf.qkv, buf.att, buf.gu, buf.slabs, ws, v.s_qkv)]
                     + [0 if v.w_qn is None else v.w_qn.data_ptr(), 0 if v.w_kn is None else v.w_kn.data_ptr()]
                     + [t_.data_ptr() for t_ in (v.s_o, v.w_ln2, v.s_gu, v.s_down, w_next)],
-                    [cache.k[l].data_ptr(), cache.v[l].data_ptr(), B, d, H, KVH, Dh, I, cache.max_len])
-            ops.decode_layer(fixed[0], self._rope_cs.data_ptr(), pos.data_ptr(), kv_len.data_ptr(), fixed[1],
-                             self._decode_split(B, t + 1), eps, int(cfg.rope_interleaved))
+                    None if mx else [cache.k[l].data_ptr(), cache.v[l].data_ptr(), B, d, H, KVH, Dh, I, cache.max_len])
+            nsplit = self._decode_split(B, t + 1, cache.fmt)
+            if mx:
+                ops.decode_layer_mx(fixed[0], self._rope_cs, pos, kv_len, cache.kv[l], B, d, H, I, nsplit, eps,
+                                    int(cfg.rope_interleaved))
+            else:
+                ops.decode_layer(fixed[0], self._rope_cs.data_ptr(), pos.data_ptr(), kv_len.data_ptr(), fixed[1], nsplit,
+                                 eps, int(cfg.rope_interleaved))
             buf.h = nxt
             return
         if buf.sk_qkv:
@@ -179,9 +277,8 @@ class GenerationMixin:
         else:
             ops.linear_fwd(buf.x, v.s_qkv, buf.qkv)
         # attention over the cache; q/k norm + rotation of the new token and its cache append happen in the same launch
-        ops.attn_decode_prep(buf.qkv, NQ, v.w_qn, v.w_kn, self._rope_cs, pos, eps, cfg.rope_interleaved, cache.k[l],
-                             cache.v[l], kv_len, buf.att, H * Dh, ws, B, H, KVH, Dh, cache.max_len,
-                             self._decode_split(B, t + 1), Dh ** -0.5)
+        cache.attend_prep(l, buf.qkv, NQ, v.w_qn, v.w_kn, self._rope_cs, pos, eps, cfg.rope_interleaved, kv_len, buf.att,
+                          H * Dh, ws, B, H, self._decode_split(B, t + 1, cache.fmt), Dh ** -0.5)
         # The two residual projections have few output tiles at M = B rows: they run split along K into fp32 slabs,
         # and one kernel sums the slabs, adds the residual and applies the norm that follows.
         if buf.sk_o:
@@ -233,8 +330,13 @@ class GenerationMixin:
                  do_sample: bool = False, temperature: float = 1.0, top_k: Optional[int] = None, top_p: float = 1.0,
                  pad_token_id: Optional[int] = None, eos_token_id: Optional[int] = None, use_cache: bool = True,
                  noise: Optional[torch.Tensor] = None, seed: int = 0, eos_check_every: int = 16,
-                 return_step_logits: bool = False, attention_mask: Optional[torch.Tensor] = None, **unused):
-        """attention_mask [B, prompt_len] (1 = real token): prompts of different lengths batched with LEFT padding, as
+                 return_step_logits: bool = False, attention_mask: Optional[torch.Tensor] = None,
+                 kv_cache: str = "bf16", **unused):
+        """kv_cache: "bf16", or "mxfp8" / "mxfp4" for a cache in blocks of 32 elements with a shared power-of-two scale
+        (8.25 / 4.25 bits an element: 1.94 / 3.76 times the streams x context in the same memory, and that much less to
+        read per decode step). The prompt's own attention runs on the unquantised keys and values.
+
+        attention_mask [B, prompt_len] (1 = real token): prompts of different lengths batched with LEFT padding, as
         transformers' generate() expects of a decoder-only model (generation/utils.py: the mask grows by a column of
         ones per token, position ids count real tokens only). Each stream then produces what it would produce alone
         from its unpadded prompt: internally the rows are shifted to start at column 0, the prefill runs on the shifted
@@ -250,6 +352,11 @@ class GenerationMixin:
             raise RuntimeError("the model carries low-rank adapters: call merge_lora() before generate(), or pass "
                                "use_cache=False")
         cfg = self.cfg
+        if kv_cache != "bf16":
+            if kv_cache not in ops.MX_BITS:
+                raise ValueError(f"kv_cache={kv_cache!r}: one of 'bf16', 'mxfp8', 'mxfp4'")
+            if not use_cache or getattr(self, "act_dtype", torch.bfloat16) == torch.float32:
+                raise ValueError(f"kv_cache={kv_cache!r} needs a KV cache: use_cache=False and the fp32 mode have none")
         B, P = input_ids.shape
         if max_new_tokens is None:
             max_new_tokens = (max_length if max_length is not None else 20) - P
@@ -330,10 +437,11 @@ class GenerationMixin:
             self._check_device_flags()
             return (out, torch.stack(step_logits, 0)) if return_step_logits else out
         held = getattr(self, "_kv_reserved", None)
-        if held is not None and B <= held.k[0].shape[0] and total <= held.max_len and held.k[0].device == dev:
+        if (held is not None and held.fmt == kv_cache and B <= held.batch and total <= held.max_len
+                and held.device == dev):
             cache = held.first_streams(B)
         else:
-            cache = KVCache(cfg, B, total, dev)
+            cache = make_kv_cache(cfg, B, total, dev, kv_cache)
         # lens[t] = int32 [B] filled with t: per-stream positions / key counts without per-step host->device traffic
         lens = torch.arange(total + 1, dtype=torch.int32, device=dev)[:, None].expand(total + 1, B).contiguous()
         if n_real is not None:   # stream b is (P - n_real[b]) positions behind the column count
@@ -349,7 +457,7 @@ class GenerationMixin:
         for i in range(nparts):
             b0, b1 = B * i // nparts, B * (i + 1) // nparts
             ws_n = ops.attn_decode_workspace(b1 - b0, cfg.num_attention_heads, cfg.head_dim,
-                                             self._decode_split(b1 - b0, total))
+                                             self._decode_split(b1 - b0, total, kv_cache))
             parts.append(_Part(cfg, cache, b0, b1, nxt_all, ws_n, dev,
                                main if nparts == 1 else torch.cuda.Stream(device=dev)))
             parts[-1].lens = lens[:, b0:b1]      # row t of the view: positions of the part's streams, contiguous
@@ -451,7 +559,7 @@ class GenerationMixin:
                     for pt in parts:
                         main.wait_stream(pt.stream)
             else:
-                key = tuple(self._decode_split(pt.b1 - pt.b0, t + 1) for pt in parts)
+                key = tuple(self._decode_split(pt.b1 - pt.b0, t + 1, kv_cache) for pt in parts)
                 g = graphs.get(key)
                 if g is None:
                     g = graphs[key] = torch.cuda.CUDAGraph()
@@ -498,7 +606,7 @@ class GenerationMixin:
         cs = self._rope4d_table(rows)
         scale = Dh ** -0.5
         pos, kv_len = lens[t], lens[t + 1]
-        nsplit = self._decode_split(B, t + 1)
+        nsplit = self._decode_split(B, t + 1, cache.fmt)
         h = buf.h0
         ops.fill_rows(self.model.embed_vector, h)
         qp = buf.rot.data_ptr()
@@ -510,9 +618,8 @@ class GenerationMixin:
             ops.linear_fwd(buf.x, v.s_qkv, buf.qkv)
             ops.qkvnorm_rope4d_fwd(buf.qkv.data_ptr(), NQ, qp, kp, vp, NQ, NQ, NQ, v.w_qn, v.w_kn, cs, B, H, KVH, KVH,
                                    Dh, eps)
-            ops.kv_append(kp, vp, NQ, NQ, cache.k[l], cache.v[l], pos, B, 1, KVH, Dh, cache.max_len)
-            ops.attn_decode(qp, NQ, cache.k[l], cache.v[l], kv_len, buf.att, H * Dh, ws, B, H, KVH, Dh, cache.max_len,
-                            nsplit, scale)
+            cache.append(l, kp, vp, NQ, NQ, pos, B, 1)
+            cache.attend(l, qp, NQ, kv_len, buf.att, H * Dh, ws, B, H, nsplit, scale)
             ops.rotate4d(buf.att, buf.att, cs, B, H, Dh, inverse=True)
             ops.linear_slabs(buf.att, v.s_o, buf.slabs, buf.ns_o)
             ops.slab_resid_rmsnorm(buf.slabs, buf.ns_o, h, buf.h1, v.w_ln2, buf.x, eps)
@@ -529,7 +636,7 @@ class GenerationMixin:
 
     @torch.no_grad()
     def generate_music(self, position_tensors, total_length: int = 200, use_cache: bool = True,
-                       return_preds: bool = False):
+                       return_preds: bool = False, kv_cache: str = "bf16"):
         """Note-by-note generation of the 4-D position model (/root/reference/generate_music.py:146-179): every
         step decodes the unit pairs predicted at the last row into [start delta, duration, pitch, velocity]
         (process_last_logits, :116-142), adds the previous start time and appends the row.
@@ -537,7 +644,8 @@ class GenerationMixin:
         position_tensors: fp32 [B, P, 4] starting rows (the reference starts from the single row
         batch['position_tensors'][0:1, 0:1]). Returns fp32 [B, P + total_length, 4].
         The reference re-runs the whole prefix for every new note; with use_cache (default) the rotated keys and
-        values stay in a pre-allocated cache and each step costs one row. use_cache=False keeps the prefix re-run."""
+        values stay in a pre-allocated cache and each step costs one row. use_cache=False keeps the prefix re-run.
+        kv_cache: the cache's type, "bf16", "mxfp8" or "mxfp4" (see generate())."""
         cfg = self.cfg
         if not cfg.pos4d:
             raise RuntimeError("generate_music() belongs to the 4-D position model (config.pos4d)")
@@ -545,6 +653,11 @@ class GenerationMixin:
             raise ValueError("position_tensors must be [batch, prompt_len >= 1, 4]")
         if not position_tensors.is_cuda:
             raise RuntimeError("MidiLM runs on the GPU only: position_tensors must be a CUDA/HIP tensor")
+        if kv_cache != "bf16":
+            if kv_cache not in ops.MX_BITS:
+                raise ValueError(f"kv_cache={kv_cache!r}: one of 'bf16', 'mxfp8', 'mxfp4'")
+            if not use_cache or getattr(self, "act_dtype", torch.bfloat16) == torch.float32:
+                raise ValueError(f"kv_cache={kv_cache!r} needs a KV cache: use_cache=False and the fp32 mode have none")
         dev = position_tensors.device
         B, P = position_tensors.shape[:2]
         total = P + total_length
@@ -570,10 +683,10 @@ class GenerationMixin:
                 decode_into(self._last_pred.data_ptr(), 16, t)
             return (out, torch.stack(preds, 1).view(B, -1, 8, 2)) if return_preds else out
 
-        cache = KVCache(cfg, B, total, dev)
+        cache = make_kv_cache(cfg, B, total, dev, kv_cache)
         buf = _DecodeBuffers(cfg, B, dev)
         lens = torch.arange(total + 1, dtype=torch.int32, device=dev)[:, None].expand(total + 1, B).contiguous()
-        ws_n = ops.attn_decode_workspace(B, cfg.num_attention_heads, cfg.head_dim, self._decode_split(B, total))
+        ws_n = ops.attn_decode_workspace(B, cfg.num_attention_heads, cfg.head_dim, self._decode_split(B, total, kv_cache))
         ws = torch.empty(max(ws_n, 1), dtype=torch.float32, device=dev)
         # prefill on the starting rows
         xN, _ = self._run_layers(out[:, :P].contiguous(), save=None, cache=cache)

@@ -162,8 +162,7 @@ class MidiGPT2LM(MidiLM):
             ops.conv1d_fwd(x1, v.s_attn, v.s_attn_b, qkv)
             qp, kp, vp = qkv.data_ptr(), qkv.data_ptr() + esz * d, qkv.data_ptr() + 2 * esz * d
             if cache is not None:
-                ops.kv_append(kp, vp, 3 * d, 3 * d, cache.k[l], cache.v[l], cache.zero_pos, B, S, H, Dh,
-                              cache.max_len)
+                cache.append(l, kp, vp, 3 * d, 3 * d, cache.zero_pos, B, S)
             att = torch.empty(T, d, dtype=bf, device=dev)
             lse = torch.empty(B, H, S, dtype=f32, device=dev)
             ops.attn_fwd(qp, kp, vp, att.data_ptr(), lse, 3 * d, 3 * d, 3 * d, d, B, S, H, H, Dh, scale, f32=full,
@@ -277,7 +276,7 @@ class MidiGPT2LM(MidiLM):
         eps = cfg.layer_norm_eps
         scale = Dh ** -0.5
         pos, kv_len = lens[t], lens[t + 1]
-        nsplit = self._decode_split(B, t + 1)
+        nsplit = self._decode_split(B, t + 1, cache.fmt)
         h = buf.h0
         ops.embed_pos_fwd(tokens, self.transformer.wte.weight, self.transformer.wpe.weight, pos, h, 1, self._err_flag)
         qp = buf.qkv.data_ptr()
@@ -286,9 +285,8 @@ class MidiGPT2LM(MidiLM):
         for l, v in enumerate(self._layers):
             ops.layernorm_fwd(h, v.w_ln1w, v.w_ln1b, buf.x, None, None, eps)
             ops.conv1d_fwd(buf.x, v.s_attn, v.s_attn_b, buf.qkv)
-            ops.kv_append(kp, vp, 3 * d, 3 * d, cache.k[l], cache.v[l], pos, B, 1, H, Dh, cache.max_len)
-            ops.attn_decode(qp, 3 * d, cache.k[l], cache.v[l], kv_len, buf.att, d, ws, B, H, H, Dh, cache.max_len,
-                            nsplit, scale)
+            cache.append(l, kp, vp, 3 * d, 3 * d, pos, B, 1)
+            cache.attend(l, qp, 3 * d, kv_len, buf.att, d, ws, B, H, nsplit, scale)
             ops.conv1d_fwd(buf.att, v.s_proj, v.s_proj_b, buf.h1, ops.OUT_F32_RESID_BF16ROUND, h)
             ops.layernorm_fwd(buf.h1, v.w_ln2w, v.w_ln2b, buf.x, None, None, eps)
             ops.conv1d_fwd(buf.x, v.s_fc, v.s_fc_b, fc)

@@ -683,7 +683,7 @@ class MidiLM(GenerationMixin, nn.Module):
                 ops.qknorm_rope_fwd(qkv, LQ, qp, kp, LK, LK, v.w_qn, v.w_kn, cs, pos, S, T, H, KVH, Dh,
                                     cfg.rms_norm_eps, interleaved=cfg.rope_interleaved)
             if cache is not None:  # prefill: rotated keys and values of every prompt position go into the cache
-                ops.kv_append(kp, vp, sk, sv, cache.k[l], cache.v[l], cache.zero_pos, B, S, KVH, Dh, cache.max_len)
+                cache.append(l, kp, vp, sk, sv, cache.zero_pos, B, S)
             apad = _ATT_PAD if (qpad and (H * Dh * esz) % 2048 == 0) else 0
             att = torch.empty(T, H * Dh + apad, dtype=bf, device=dev)[:, :H * Dh]
             lse = torch.empty(B, H, S, dtype=torch.float32, device=dev)

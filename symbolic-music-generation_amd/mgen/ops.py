@@ -730,6 +730,14 @@ def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_le
          ld_o, _mx_workspace(workspace, B, H, D, nsplit), B, H, kv.KVH, D, kv.max_len, kv.bits, nsplit, scale, _stream())
 
 
+def decode_layer_mx(ptrs17, cs, pos, kv_len, kv, B, d, H, I, nsplit, eps, interleaved):
+    """decode_layer over a quantised cache (an MXKV): ptrs17 as there; cs is the rotary table [positions, D/2, 2], pos and
+    kv_len int32 tensors of at least B entries."""
+    kv._check(B, pos=pos, kv_len=kv_len)
+    call("mgen_decode_layer_mx", *ptrs17, _p(cs), cs.shape[0], _p(pos), _p(kv_len), *kv.ptrs, B, d, H, kv.KVH, kv.D, I,
+         kv.max_len, kv.bits, nsplit, eps, interleaved, _stream())
+
+
 def sample(logits, V, out, do_sample=False, temperature=1.0, top_k=0, top_p=1.0, noise=None, seed=0, offset=0,
            out2=None, out2_stride=0, row0=0, step=None, unfinished=None, eos_id=0, pad_id=0):
     """logits [B, ld] (bf16 or fp32) -> out [B] int64; out2 = raw pointer of an optional strided second destination.

@@ -8,19 +8,30 @@
 //
 // Bound: HBM. A key and its value are 2 (D/2 + D/32) bytes in 4 bits, read once for all query heads of their kv head.
 //
-// One workgroup per (key split, kv head with up to 4 query heads, stream); a wave walks tiles of 16 keys. Lane (r, g),
-// r = lane & 15, g = lane >> 4, takes the g-th quarter of key r's row: a tile is one contiguous run of memory and the
-// quarter lies in one block, so a lane needs one scale byte per row.
-//  * Scores on the matrix cores: the codes become bf16 fragments (exactly) as they come from memory; the reduction
-//    index of fragment j runs over elements 8j .. 8j+7 of every quarter, a permutation that q shares. Query head i sits
-//    in rows i, 4 + i, 8 + i, 12 + i of the other operand, so that every lane finds the scores of ITS key r for all heads
-//    in its own accumulator: no exchange between lanes anywhere in the loop.
-//  * Values on the vector unit: a lane's quarter of V_r as fp32, weighted into D/4 accumulators per head. Each lane keeps
-//    the sum over its own keys; the 16 lanes of a row meet once, after the loop.
-//  * The running maximum is one number per wave and head and moves only when a score exceeds it by more than 2^8 in the
-//    weight (sums stay far inside fp32); then the sums are scaled. Weights, sums and outputs are fp32.
-//  * Rows outside the split are never read: the loads go through buffer descriptors that end at the split's last key and
-//    give zeros behind it (codes and scale: the value 0), and their weights are set to 0.
+// One workgroup per (key split, kv head with up to 8 query heads, stream); its waves walk units of keys.
+//
+// One query head per kv head (MXOne), all on the vector unit: a load instruction is one contiguous kilobyte, 16 bytes of
+// codes per lane (32 or 16 elements of one key, in one block), LR = 2, 4 or 8 lanes per row. Scores: codes to bf16 pairs,
+// two products and their sum per instruction, the LR lanes of a row add up. V: codes to fp32, weighted into the lane's own
+// sums (its elements, over its own keys). Keys meet after the loop.
+//
+// Several query heads (MXHeads), on the matrix cores: a wave walks two tiles of 16 keys; lane (r, g), r = lane & 15, g =
+// lane >> 4, takes the g-th quarter of key r's row, and its codes become bf16 operand fragments of 8 elements (exactly).
+//  * Scores: the reduction runs over the elements in the order the lanes hold them, a permutation that q shares. The heads
+//    are the columns (columns i and 8 + i hold the same head): lane (r, g) ends up with column r, keys 4g .. 4g+3, which is
+//    the operand layout of the second product, so the weights never cross lanes.
+//  * The second product reduces over keys, so a lane needs V by element, not by key: the matrix cores turn the tile around
+//    (V fragment times a 0/1 selection of 16 of its 32 elements - one product per output, exact), a matrix instruction per
+//    16 x 16 elements of a pipe that is mostly idle here, instead of a round trip through LDS.
+//  * Weights enter as two bf16 numbers, their rounded value in columns 0..7 and what that leaves in columns 8..15 (16 bits
+//    of weight at the price of 8); the two rows are added at the end.
+//  * A value block written with an infinity or a NaN enters as zeros and its elements of the result are set to NaN at the
+//    end (0 * NaN in the turning product would reach the other elements).
+//
+// Both: the running maximum of a head is shared by the wave and moves only when a score exceeds it by more than 2^8 in the
+// weight (sums stay far inside fp32); then the sums are scaled. Sums, maxima and outputs are fp32. Rows outside the split
+// are never read: the loads go through buffer descriptors that end at the split's last key and give zeros behind it (codes
+// and scale: the value 0), and the weights of the last unit of keys are masked.
 #include "kvmx.h"
 #include "decode_prep.h"
 
@@ -29,6 +40,7 @@ namespace {
 constexpr float MX_LOG2E = 1.4426950408889634f;
 constexpr float MX_LOW = -3.0e38f;      // below every finite score that matters; not -inf, so that differences stay numbers
 constexpr float MX_SLACK = 8.0f;
+constexpr int MX_HEADS = 8;            // query heads of a workgroup
 
 struct MXView {
     const unsigned char *k, *ks, *v, *vs;
@@ -49,50 +61,344 @@ __device__ __forceinline__ rsrc_t mx_rsrc(const unsigned char* p, unsigned bytes
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, (int)bytes, 0x00020000);
 }
 
-// a lane's quarter of a row: W dwords
-template <int W>
-__device__ __forceinline__ void mx_load(rsrc_t r, int off, unsigned* out) {
-    if (W == 2) {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
-        out[0] = v[0]; out[1] = v[1];
-    } else {
+struct MXRsrc {                          // the split's keys: codes and scales of K and V
+    rsrc_t k, ks, v, vs;
+};
+__device__ __forceinline__ u32x4 mx_load16(rsrc_t r, int off, bool stream) {
+    return stream ? __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 2) : __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+}
+__device__ __forceinline__ f32x4 mx_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// A core holds T tiles of KPT keys per unit: codes k[T], v[T] (W dwords) and scale bytes ke[T], ve[T] of its lane's part of
+// each row (NP pieces, each inside one block), and the softmax state of its wave.
+
+// One query head
+template <int D, int BITS>
+struct MXOne {
+    static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
+    static constexpr int LR = RB / 16;                // lanes of a row
+    static constexpr int KPT = 64 / LR, T = 4, W = 4, NP = 1;
+    static constexpr int ED = 128 / BITS;             // elements of a lane
+    static constexpr int WF = BITS / 4;               // dwords of 8 elements
+    static constexpr int PARTS = 4;                   // results a wave leaves for a head: one per 16 lanes
+
+    unsigned k[T][W], v[T][W], ke[T], ve[T];
+    bf16x2 q[ED / 2];
+    float m, l, acc[ED], sl2;
+    int lane;
+
+    __device__ __forceinline__ void place(int lane_) { lane = lane_; }
+    __device__ __forceinline__ int key() const { return lane / LR; }                       // of a tile
+    __device__ __forceinline__ int elem(int j) const { return lane % LR * ED + 8 * j; }    // of the lane's j-th eight
+    __device__ __forceinline__ int block(int) const { return lane % LR * ED / 32; }
+
+    __device__ __forceinline__ void start(const bf16* src, int nh, float scale_log2e) {
+        sl2 = scale_log2e;
 #pragma unroll
-        for (int h = 0; h < W / 4; ++h) {
-            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * h, 0, 0);
+        for (int j = 0; j < ED / 8; ++j) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(src + elem(j));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[4 * h + i] = v[i];
+            for (int i = 0; i < 4; ++i) {
+                const unsigned w = x[i];
+                q[4 * j + i] = mx_pair(w);
+            }
+        }
+        m = MX_LOW;
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < ED; ++e) acc[e] = 0.f;
+    }
+    __device__ __forceinline__ void load(const MXRsrc& s, int base) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int at = base + t * KPT;
+            ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at * NB + key() * NB + block(0), 0, 0);
+            ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at * NB + key() * NB + block(0), 0, 0);
+            const u32x4 x = mx_load16(s.k, at * RB + lane * 16, true), y = mx_load16(s.v, at * RB + lane * 16, true);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                k[t][i] = x[i];
+                v[t][i] = y[i];
+            }
         }
     }
-}
+    // left: keys from the unit's first on (LAST: fewer than T * KPT may be there)
+    template <bool LAST>
+    __device__ __forceinline__ void unit(int left) {
+        float s[T], mx = MX_LOW;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const float sc = mx_scale(ke[t]);
+            float d[2] = {0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < ED / 8; ++j) {
+                const u32x4 x = __builtin_bit_cast(u32x4, mx_decode8<BITS>(k[t] + j * WF, sc));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned w = x[i];
+                    d[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(mx_pair(w), q[4 * j + i], d[i & 1], false);
+                }
+            }
+            float a = d[0] + d[1];
+            a += dppf_xor1(a);
+            if (LR >= 4) a += dppf_xor2(a);
+            if (LR >= 8) a += dppf_xor7(a);
+            s[t] = a * sl2;
+            if (LAST) s[t] = t * KPT + key() < left ? s[t] : MX_LOW;
+            mx = fmaxf(mx, s[t]);
+        }
+        if (__any(mx > m + MX_SLACK)) {
+            float top = row16_max(mx);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
+            const float alpha = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= alpha;
+#pragma unroll
+            for (int e = 0; e < ED; ++e) acc[e] *= alpha;
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            float w = __builtin_amdgcn_exp2f(s[t] - m);
+            if (LAST) w = t * KPT + key() < left ? w : 0.f;
+            l += w;
+            const float sc = mx_scale(ve[t]);
+#pragma unroll
+            for (int x = 0; x < W; ++x) {
+                constexpr int PW = 32 / BITS;
+                float f[PW];
+                mx_decode_f32<BITS>(v[t][x], sc, f);
+#pragma unroll
+                for (int e = 0; e < PW; ++e) acc[x * PW + e] = fmaf(w, f[e], acc[x * PW + e]);
+            }
+        }
+    }
+    // sum over the keys of a row of 16 lanes: lanes that hold the same elements are LR apart
+    __device__ __forceinline__ static float keys_sum(float x) {
+        if (LR <= 2) x += dppf_ror2(x);
+        if (LR <= 4) x += dppf_ror4(x);
+        return x + dppf_ror8(x);
+    }
+    // maximum, denominator and sums of the wave's four rows of lanes to ml[4][2] and o[4][D]
+    __device__ __forceinline__ void finish(float* ml, float* o, int nh, int hc) {
+        l = keys_sum(l);
+#pragma unroll
+        for (int e = 0; e < ED; ++e) acc[e] = keys_sum(acc[e]);
+        const int row = lane >> 4;
+        if ((lane & 15) < LR) {
+#pragma unroll
+            for (int e = 0; e < ED; e += 4)
+                *reinterpret_cast<f32x4*>(o + row * D + (lane & 15) * ED + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+        }
+        if ((lane & 15) == 0) {
+            ml[2 * row] = m;
+            ml[2 * row + 1] = l;
+        }
+    }
+};
+
+// Up to MX_HEADS query heads. A lane's quarter of a row comes in NP pieces of at most 16 bytes: a load instruction takes
+// piece p of all 16 rows of a tile, 64 (32) contiguous bytes of every row.
+template <int D, int BITS>
+struct MXHeads {
+    static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
+    static constexpr int KPT = 16, T = 2, W = RB / 16;
+    static constexpr int NP = RB == 128 ? 2 : 1;
+    static constexpr int PB = RB / 4 / NP;            // bytes of a piece
+    static constexpr int PD = D / 4 / NP;             // elements of a piece
+    static constexpr int NF = D / 32;                 // fragments of 8 elements
+    static constexpr int WF = BITS / 4;               // dwords of a fragment
+    static constexpr int PARTS = 1;
+
+    unsigned k[T][W], v[T][W], ke[T], ve[T];          // ke, ve: one byte, or with two pieces the row's four
+    bf16x8 qf[NF], pick[2];
+    float m, l, sl2, low;                 // of column r; low: the column takes the weights' remainders
+    f32x4 acc[NF][2];                     // rows = columns of the scores, column r of selection c
+    unsigned long long bad[NP];           // lanes that met a value block of scale 255, by piece
+    int r, g;
+
+    __device__ __forceinline__ void place(int lane) {
+        r = lane & 15;
+        g = lane >> 4;
+    }
+    __device__ __forceinline__ int key() const { return r; }
+    __device__ __forceinline__ static int elem_of(int j, int g) { return (j * 8 / PD) * 4 * PD + g * PD + j * 8 % PD; }
+    __device__ __forceinline__ int elem(int j) const { return elem_of(j, g); }
+    __device__ __forceinline__ int block(int p) const { return (p * 4 * PD + g * PD) / 32; }
+    __device__ __forceinline__ unsigned byte(unsigned e, int p) const { return NP == 1 ? e : (e >> (8 * block(p))) & 255u; }
+
+    __device__ __forceinline__ void start(const bf16* q, int nh, float scale_log2e) {
+        sl2 = scale_log2e;
+        low = r >> 3 ? 1.f : 0.f;
+        m = MX_LOW;
+        l = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) bad[p] = 0;
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            qf[j] = bf16x8{};
+            if ((r & 7) < nh) qf[j] = *reinterpret_cast<const bf16x8*>(q + (r & 7) * D + elem(j));
+        }
+        // selection c: column r of the turned tile is element r & 7 of the fragment of lanes g = 2c + (r >> 3)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pick[c][e] = (bf16)(g == 2 * c + (r >> 3) && e == (r & 7) ? 1.f : 0.f);
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) acc[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ static void load_row(rsrc_t s, int off, unsigned* out) {
+        if (W == 2) {
+            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(s, off, 0, 0);
+            out[0] = x[0];
+            out[1] = x[1];
+        } else {
+#pragma unroll
+            for (int h = 0; h < W / 4; ++h) {
+                const u32x4 x = mx_load16(s, off + 4 * PB * h, false);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[4 * h + i] = x[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const MXRsrc& s, int base) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int at = base + 16 * t + r;
+            if (NP == 1) {
+                ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at * NB + block(0), 0, 0);
+                ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at * NB + block(0), 0, 0);
+            } else {
+                ke[t] = __builtin_amdgcn_raw_buffer_load_b32(s.ks, at * NB, 0, 0);
+                ve[t] = __builtin_amdgcn_raw_buffer_load_b32(s.vs, at * NB, 0, 0);
+            }
+            load_row(s.k, at * RB + g * PB, k[t]);
+            load_row(s.v, at * RB + g * PB, v[t]);
+        }
+    }
+    template <bool LAST>
+    __device__ __forceinline__ void unit(int left) {
+        float s[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+                a = mx_mfma(mx_decode8<BITS>(k[t] + j * WF, mx_scale(byte(ke[t], j * 8 / PD))), qf[j], a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[4 * t + i] = a[i] * sl2;
+                if (LAST) s[4 * t + i] = 16 * t + 4 * g + i < left ? s[4 * t + i] : MX_LOW;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+        if (__any(mx > m + MX_SLACK)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m);
+            const float alpha = __builtin_amdgcn_exp2f(m - mx);
+            m = mx;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float row = __shfl(alpha, 4 * g + i, 64);     // of the column that row 4g + i of the sums belongs to
+#pragma unroll
+                for (int j = 0; j < NF; ++j) {
+                    acc[j][0][i] *= row;
+                    acc[j][1][i] *= row;
+                }
+            }
+        }
+        bf16x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float w = __builtin_amdgcn_exp2f(s[i] - m);
+            if (LAST) w = 16 * (i >> 2) + 4 * g + (i & 3) < left ? w : 0.f;
+            l += w;
+            p[i] = (bf16)fmaf(-low, round_bf(w), w);
+        }
+        float vs[2][NP];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < NP; ++x) {
+                const unsigned e = byte(ve[t], x);
+                bad[x] |= __ballot(e == 255u);
+                vs[t][x] = e == 255u ? 0.f : mx_scale(e);
+            }
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            const bf16x8 v0 = mx_decode8<BITS>(v[0] + j * WF, vs[0][j * 8 / PD]);
+            const bf16x8 v1 = mx_decode8<BITS>(v[1] + j * WF, vs[1][j * 8 / PD]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                const f32x4 t0 = mx_mfma(v0, pick[c], zero), t1 = mx_mfma(v1, pick[c], zero);   // keys 4g + i, column r
+                bf16x8 x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = (bf16)t0[i];
+                    x[4 + i] = (bf16)t1[i];
+                }
+                acc[j][c] = mx_mfma(p, x, acc[j][c]);
+            }
+        }
+    }
+    __device__ __forceinline__ void finish(float* ml, float* o, int nh, int hc) {
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0 && r < nh) {
+            ml[2 * r] = m;
+            ml[2 * r + 1] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int from = 2 * c + (r >> 3);                  // lanes g the column's element came from
+                const float nan = (bad[j * 8 / PD] >> (16 * from)) & 0xFFFFu ? __uint_as_float(0x7FC00000u) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {                       // rows 8 + i hold the remainders
+                    const float x = acc[j][c][i] + __shfl_xor(acc[j][c][i], 32, 64) + nan;
+                    if (4 * g + i < nh) o[(4 * g + i) * D + elem_of(j, from) + (r & 7)] = x;
+                }
+            }
+    }
+};
 
 // PREP = 0: q is ready in `q` and the cache holds kv_len[b] keys. PREP = 1 (split-half pairs) / 2 (adjacent pairs): q,
 // the new key and the new value come from the raw projection rows; the new row is quantised, takes the place of key
 // kv_len[b] - 1 in the lanes that own it, and is written to the cache by the first head group.
-// GC: query heads of the workgroup; U: tiles a wave has in flight; NW: waves
-template <int D, int BITS, int GC, int PREP, int U, int NW>
+template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
                                                                  const int* __restrict__ kv_len, int H, int KVH,
                                                                  int nsplit, float scale, float* __restrict__ part_ml,
                                                                  float* __restrict__ part_o, bf16* __restrict__ out,
                                                                  long ld_o, MXPrep pp) {
-    constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
-    constexpr int W = RB / 16;            // dwords of a quarter row
-    constexpr int NF = D / 32;            // bf16 fragments of a quarter row
-    constexpr int ND = D / 4;             // elements of a quarter row
-    __shared__ float sm_ml[NW * GC * 2];
-    __shared__ __attribute__((aligned(16))) float sm_o[NW * GC * D];
-    __shared__ __attribute__((aligned(16))) bf16 sm_new[PREP ? (GC + 2) * D : 8];   // q heads, new key, new value
+    typedef Core<D, BITS> C;
+    constexpr int RB = C::RB, NB = C::NB, KPT = C::KPT, KPU = C::T * KPT, NR = NW * C::PARTS;
+    extern __shared__ __attribute__((aligned(16))) float smem[];
 
-    const int group = H / KVH, chunks = (group + GC - 1) / GC;
+    const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS;
     const int split = blockIdx.x, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
-    const int h0 = kvh * group + chunk * GC, nh = min(GC, group - chunk * GC);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r = lane & 15, g = lane >> 4;
+    const int h0 = kvh * group + chunk * MX_HEADS, nh = min(MX_HEADS, group - chunk * MX_HEADS), hc = min(MX_HEADS, group);
+    bf16* sm_q = reinterpret_cast<bf16*>(smem);      // [hc + 2][D]: q heads, new key, new value (PREP); gives way to
+    float* sm_o = smem;                              // [NW][PARTS or heads][D] and
+    float* sm_ml = smem + NR * hc * D;               // [NW][PARTS or heads][2]
+    const int tid = threadIdx.x, wave = tid >> 6;
+    C core;
+    core.place(tid & 63);
 
     int len = min(kv_len[b], kv.max_len);
     const int pos = PREP ? pp.pos[b] : 0;
     if (PREP && (pos < 0 || pos >= kv.max_len || pos >= pp.npos || kv_len[b] != pos + 1)) len = 0;
     if (len <= 0) {                       // a stream without keys: zeros
+#pragma unroll 1
         for (int i = tid; i < nh * D; i += 64 * NW) {
             const int h = h0 + i / D;
             if (nsplit == 1) out[(long)b * ld_o + (long)h * D + i % D] = (bf16)0.f;
@@ -104,190 +410,97 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const bf16* __r
         }
         return;
     }
-    const int per = ((len + nsplit - 1) / nsplit + 15) & ~15;
+    const int per = ((len + nsplit - 1) / nsplit + 31) & ~31;
     const int k_beg = (int)min((long)split * per, (long)len), n = min(len - k_beg, per);     // keys of this split
-    const int k_new = PREP ? len - 1 - k_beg : -1;                  // the new key, counted from k_beg
+
+    const long slice = ((long)b * KVH + kvh) * kv.max_len;
+    const unsigned nk = (unsigned)n;
+    const MXRsrc src{mx_rsrc(kv.k + (slice + k_beg) * RB, nk * RB), mx_rsrc(kv.ks + (slice + k_beg) * NB, nk * NB),
+                     mx_rsrc(kv.v + (slice + k_beg) * RB, nk * RB), mx_rsrc(kv.vs + (slice + k_beg) * NB, nk * NB)};
 
     if (PREP) {
         constexpr int L16 = D / 16;
-        if (tid < (GC + 2) * L16) {
-            const int which = tid / L16, s16 = tid % L16;
-            const bf16* row = pp.qkv + (long)b * pp.ld_in;
-            const float* csr = pp.cs + (long)pos * D;
-            if (which < GC) {
-                if (which < nh) prep_row<D, PREP == 2>(row + (long)(h0 + which) * D, pp.wq, csr, pp.eps, s16, sm_new + which * D);
-            } else if (which == GC)
-                prep_row<D, PREP == 2>(row + (long)(H + kvh) * D, pp.wk, csr, pp.eps, s16, sm_new + GC * D);
-            else {
+        const int s16 = tid % L16;
+        const bf16* row = pp.qkv + (long)b * pp.ld_in;
+        const float* csr = pp.cs + (long)pos * D;
+#pragma unroll 1
+        for (int which = tid / L16; which < nh + 2; which += 64 * NW / L16) {
+            if (which < nh + 1) {
+                const bool isq = which < nh;
+                prep_row<D, PREP == 2>(row + (long)(isq ? h0 + which : H + kvh) * D, isq ? pp.wq : pp.wk, csr, pp.eps, s16,
+                                       sm_q + (isq ? which : hc) * D);
+            } else {
                 const bf16* src = row + (long)(H + KVH + kvh) * D + 16 * s16;
-                bf16* dst = sm_new + (GC + 1) * D + 16 * s16;
+                bf16* dst = sm_q + (hc + 1) * D + 16 * s16;
                 *reinterpret_cast<bf16x8*>(dst) = *reinterpret_cast<const bf16x8*>(src);
                 *reinterpret_cast<bf16x8*>(dst + 8) = *reinterpret_cast<const bf16x8*>(src + 8);
             }
         }
         __syncthreads();
     }
+    core.start(PREP ? sm_q : q + (long)b * ld_q + (long)h0 * D, nh, scale * MX_LOG2E);
 
-    // q: rows i, 4 + i, 8 + i, 12 + i of the operand hold head h0 + i (zeros from nh on)
-    bf16x8 qf[NF];
-    {
-        const int i = r & 3;
-        const bf16* src = PREP ? sm_new + i * D : q + (long)b * ld_q + (long)(h0 + i) * D;
-#pragma unroll
-        for (int j = 0; j < NF; ++j) {
-            qf[j] = bf16x8{};
-            if (i < nh) qf[j] = *reinterpret_cast<const bf16x8*>(src + g * ND + 8 * j);
-        }
+    int base = wave * KPU;
+#pragma unroll 1
+    for (; base + KPU < n; base += NW * KPU) {       // units before the one with the split's last key
+        core.load(src, base);
+        core.template unit<false>(0);
     }
-    const long slice = ((long)b * KVH + kvh) * kv.max_len;
-    const unsigned nk = (unsigned)max(n, 0);
-    const rsrc_t rk = mx_rsrc(kv.k + (slice + k_beg) * RB, nk * RB), rv = mx_rsrc(kv.v + (slice + k_beg) * RB, nk * RB);
-    const rsrc_t rks = mx_rsrc(kv.ks + (slice + k_beg) * NB, nk * NB), rvs = mx_rsrc(kv.vs + (slice + k_beg) * NB, nk * NB);
-    const int blk = g * NB / 4;           // block of this lane's quarter
-    const float sl2 = scale * MX_LOG2E;
-
-    float m[GC], l[GC], acc[GC][ND];
+    if (base < n) {
+        core.load(src, base);
+        const int t_new = n - 1 - base;   // the stream's last key, in its last split
+        if (PREP && k_beg + n == len && core.key() == t_new % KPT) {
 #pragma unroll
-    for (int i = 0; i < GC; ++i) {
-        m[i] = MX_LOW;
-        l[i] = 0.f;
+            for (int which = 0; which < 2; ++which) {
+                const bf16* row = sm_q + (hc + which) * D;
+                unsigned char* codes = const_cast<unsigned char*>(which ? kv.v : kv.k) + (slice + pos) * RB;
+                unsigned char* scales = const_cast<unsigned char*>(which ? kv.vs : kv.ks) + (slice + pos) * NB;
+                unsigned c[C::W], all = 0;
 #pragma unroll
-        for (int e = 0; e < ND; ++e) acc[i][e] = 0.f;
-    }
-
-    for (int base = wave * 16 * U; base < n; base += NW * 16 * U) {
-        unsigned kk[U][W], vv[U][W], ke[U], ve[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int key = base + 16 * u + r;
-            ke[u] = __builtin_amdgcn_raw_buffer_load_b8(rks, key * NB + blk, 0, 0);
-            mx_load<W>(rk, key * RB + g * (RB / 4), kk[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int key = base + 16 * u + r;
-            ve[u] = __builtin_amdgcn_raw_buffer_load_b8(rvs, key * NB + blk, 0, 0);
-            mx_load<W>(rv, key * RB + g * (RB / 4), vv[u]);
-        }
-        if (PREP && k_new >= base && k_new < base + 16 * U) {       // (the same for all lanes of the wave)
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (base + 16 * u + r != k_new) continue;
-#pragma unroll
-                for (int which = 0; which < 2; ++which) {
-                    const bf16* row = sm_new + (GC + which) * D;
+                for (int j = 0; j < C::W / C::WF; ++j) {
+                    constexpr int PER = C::W / C::WF / C::NP;       // eights of a piece
+                    const int blk = core.block(j / PER);
                     unsigned top = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        top = max(top, mx_top8(*reinterpret_cast<const bf16x8*>(row + 32 * blk + 8 * j)));
+                    for (int i = 0; i < 4; ++i)
+                        top = max(top, mx_top8(*reinterpret_cast<const bf16x8*>(row + 32 * blk + 8 * i)));
                     const unsigned e = mx_exponent<BITS>(top);
-                    unsigned* c = which ? vv[u] : kk[u];
-#pragma unroll
-                    for (int j = 0; j < NF; ++j)
-                        mx_encode8<BITS>(*reinterpret_cast<const bf16x8*>(row + g * ND + 8 * j), e, c + j * (BITS / 4));
-                    (which ? ve : ke)[u] = e;
+                    mx_encode8<BITS>(*reinterpret_cast<const bf16x8*>(row + core.elem(j)), e, c + j * C::WF);
+                    if (j % PER == 0) all |= C::NP == 1 ? e : e << (8 * blk);
                     if (chunk == 0) {
-                        unsigned char* codes = const_cast<unsigned char*>(which ? kv.v : kv.k) + (slice + pos) * RB + g * (RB / 4);
 #pragma unroll
-                        for (int j = 0; j < W; j += 2) *reinterpret_cast<u32x2*>(codes + 4 * j) = u32x2{c[j], c[j + 1]};
-                        // (quarters that share a block write the same byte)
-                        const_cast<unsigned char*>(which ? kv.vs : kv.ks)[(slice + pos) * NB + blk] = (unsigned char)e;
+                        for (int x = 0; x < C::WF; ++x)
+                            *reinterpret_cast<unsigned*>(codes + core.elem(j) * BITS / 8 + 4 * x) = c[j * C::WF + x];
+                        scales[blk] = (unsigned char)e;             // (lanes that share a block write the same byte)
                     }
                 }
+#pragma unroll
+                for (int t = 0; t < C::T; ++t)
+                    if (t == t_new / KPT) {
+#pragma unroll
+                        for (int x = 0; x < C::W; ++x) (which ? core.v : core.k)[t][x] = c[x];
+                        (which ? core.ve : core.ke)[t] = all;
+                    }
             }
         }
-        float s[U][GC], mx[GC];
-#pragma unroll
-        for (int i = 0; i < GC; ++i) mx[i] = MX_LOW;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float sc = mx_scale(ke[u]);
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < NF; ++j)
-                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[j], mx_decode8<BITS>(kk[u] + j * (BITS / 4), sc), a, 0, 0, 0);
-            const bool in = base + 16 * u + r < n;
-#pragma unroll
-            for (int i = 0; i < GC; ++i) {
-                s[u][i] = in ? a[i] * sl2 : MX_LOW;
-                mx[i] = fmaxf(mx[i], s[u][i]);
-            }
-        }
-        bool grow = false;
-#pragma unroll
-        for (int i = 0; i < GC; ++i) grow |= mx[i] > m[i] + MX_SLACK;
-        if (__any(grow)) {
-#pragma unroll
-            for (int i = 0; i < GC; ++i) {
-                const float top = fmaxf(m[i], row16_max(mx[i]));
-                const float alpha = __builtin_amdgcn_exp2f(m[i] - top);
-                m[i] = top;
-                l[i] *= alpha;
-#pragma unroll
-                for (int e = 0; e < ND; ++e) acc[i][e] *= alpha;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = base + 16 * u + r < n;
-            const float sc = mx_scale(ve[u]);
-#pragma unroll
-            for (int i = 0; i < GC; ++i) {
-                s[u][i] = in ? __builtin_amdgcn_exp2f(s[u][i] - m[i]) : 0.f;
-                l[i] += s[u][i];
-            }
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                constexpr int PW = 32 / BITS;
-                float f[PW];
-                mx_decode_f32<BITS>(vv[u][w], sc, f);
-#pragma unroll
-                for (int i = 0; i < GC; ++i)
-#pragma unroll
-                    for (int e = 0; e < PW; ++e) acc[i][w * PW + e] = fmaf(s[u][i], f[e], acc[i][w * PW + e]);
-            }
-        }
+        core.template unit<true>(n - base);
     }
 
-    // The 16 lanes of a row: sums over their keys, halving the elements a lane is responsible for at every step (lane r
-    // ends up with elements r * ND/16 ... of quarter g). A step pairs lanes whose lower bits are mirrored; bits already
-    // used stay equal.
-#pragma unroll
-    for (int i = 0; i < GC; ++i) {
-        const float ls = row16_sum(l[i]);
-        float t[ND];
-#pragma unroll
-        for (int e = 0; e < ND; ++e) t[e] = acc[i][e];
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            const int half = ND >> (st + 1);
-            const bool up = r & (8 >> st);
-#pragma unroll
-            for (int e = 0; e < half; ++e) {
-                const float keep = up ? t[e + half] : t[e], give = up ? t[e] : t[e + half];
-                t[e] = keep + (st == 0 ? dppf_xor15(give) : st == 1 ? dppf_xor7(give) : st == 2 ? dppf_xor3(give) : dppf_xor1(give));
-            }
-        }
-        float* o = sm_o + (wave * GC + i) * D + g * ND + r * (ND / 16);
-#pragma unroll
-        for (int e = 0; e < ND / 16; ++e) o[e] = t[e];
-        if (lane == 0) {
-            sm_ml[(wave * GC + i) * 2] = m[i];
-            sm_ml[(wave * GC + i) * 2 + 1] = ls;
-        }
-    }
+    if (PREP) __syncthreads();            // sm_q lies where the sums go
+    core.finish(sm_ml + wave * C::PARTS * hc * 2, sm_o + wave * C::PARTS * hc * D, nh, hc);
     __syncthreads();
+#pragma unroll 1
     for (int x = tid; x < nh * D; x += 64 * NW) {
         const int i = x / D, d = x % D;
         float M = MX_LOW;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_ml[(w * GC + i) * 2]);
+        for (int w = 0; w < NR; ++w) M = fmaxf(M, sm_ml[(w * hc + i) * 2]);
         float L = 0.f, o = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sm_ml[(w * GC + i) * 2] - M);
-            L += sm_ml[(w * GC + i) * 2 + 1] * f;
-            o += sm_o[(w * GC + i) * D + d] * f;
+        for (int w = 0; w < NR; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sm_ml[(w * hc + i) * 2] - M);
+            L += sm_ml[(w * hc + i) * 2 + 1] * f;
+            o += sm_o[(w * hc + i) * D + d] * f;
         }
         if (nsplit == 1) out[(long)b * ld_o + (long)(h0 + i) * D + d] = (bf16)(o / L);
         else {
@@ -319,21 +532,17 @@ __global__ void attn_decode_mx_merge_kernel(const float* __restrict__ part_ml, c
 
 constexpr int MX_MAX_SPLITS = 64;
 
-int heads_per_group(int H, int KVH) {
-    const int group = H / KVH;
-    return group == 1 ? 1 : group == 2 ? 2 : 4;
-}
-
-template <int D, int BITS, int GC, int PREP>
+template <int D, int BITS, int PREP, template <int, int> class Core>
 void launch(const void* q, long ld_q, MXView kv, const int* kv_len, void* out, long ld_o, float* ws, int B, int H,
             int KVH, int nsplit, float scale, MXPrep pp, hipStream_t stream) {
-    constexpr int NW = 4, U = D * BITS / 8 == 128 ? 2 : 4;
+    constexpr int NW = 4, PARTS = Core<D, BITS>::PARTS;
     float* part_ml = ws;
     float* part_o = ws ? ws + (long)B * H * nsplit * 2 : nullptr;
-    const int chunks = (H / KVH + GC - 1) / GC;
-    hipLaunchKernelGGL((attn_decode_mx_kernel<D, BITS, GC, PREP, U, NW>), dim3(nsplit, KVH * chunks, B), dim3(64 * NW), 0,
-                       stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, scale, part_ml, part_o, (bf16*)out,
-                       ld_o, pp);
+    const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS, hc = group < MX_HEADS ? group : MX_HEADS;
+    const int lds = NW * PARTS * hc * (D + 2) * 4;   // (more than the PREP rows: (hc + 2) * D * 2 bytes)
+    hipLaunchKernelGGL((attn_decode_mx_kernel<D, BITS, PREP, Core, NW>), dim3(nsplit, KVH * chunks, B), dim3(64 * NW), lds,
+                       stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, scale, part_ml, part_o, (bf16*)out, ld_o,
+                       pp);
     if (nsplit > 1)
         hipLaunchKernelGGL((attn_decode_mx_merge_kernel<D>), dim3(H, B), dim3(D), 0, stream, part_ml, part_o, nsplit, H,
                            (bf16*)out, ld_o);
@@ -356,13 +565,10 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
     MGEN_REQUIRE((((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, "%s: codes must be 16-byte aligned", what);
     const MXView kv{(const unsigned char*)kc, (const unsigned char*)ks, (const unsigned char*)vc,
                     (const unsigned char*)vs, max_len};
-#define LAUNCH(DD, BB)                                                                                                \
-    do {                                                                                                              \
-        switch (heads_per_group(H, KVH)) {                                                                            \
-            case 1: launch<DD, BB, 1, PREP>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); break;  \
-            case 2: launch<DD, BB, 2, PREP>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); break;  \
-            default: launch<DD, BB, 4, PREP>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream);        \
-        }                                                                                                             \
+#define LAUNCH(DD, BB)                                                                                                 \
+    do {                                                                                                               \
+        if (H == KVH) launch<DD, BB, PREP, MXOne>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
+        else launch<DD, BB, PREP, MXHeads>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream);  \
     } while (0)
     if (D == 128) { if (bits == 4) LAUNCH(128, 4); else LAUNCH(128, 8); }
     else { if (bits == 4) LAUNCH(64, 4); else LAUNCH(64, 8); }
@@ -375,7 +581,7 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 // Key splits for a call whose longest stream has `longest` keys
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
     if (B <= 0 || KVH <= 0 || H < KVH || longest <= 0) return 1;
-    const int GC = heads_per_group(H, KVH), chunks = (H / KVH + GC - 1) / GC;
+    const int chunks = (H / KVH + MX_HEADS - 1) / MX_HEADS;
     const long groups = (long)B * KVH * chunks;
     const long want = (1024 + groups - 1) / groups, most = (longest + 255) / 256;
     const long n = groups >= 1024 ? 1 : want < most ? want : most;

@@ -109,6 +109,9 @@ __device__ __forceinline__ int dpp_xor2(int v) { return __builtin_amdgcn_update_
 __device__ __forceinline__ int dpp_xor3(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x1B, 0xF, 0xF, true); }
 __device__ __forceinline__ int dpp_xor7(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true); }   // 7 - i in 8
 __device__ __forceinline__ int dpp_xor15(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true); }  // 15 - i
+__device__ __forceinline__ float dppf_ror2(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xF, 0xF, true)); }
+__device__ __forceinline__ float dppf_ror4(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xF, 0xF, true)); }
+__device__ __forceinline__ float dppf_ror8(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true)); }
 __device__ __forceinline__ float dppf_xor1(float v) { return __int_as_float(dpp_xor1(__float_as_int(v))); }
 __device__ __forceinline__ float dppf_xor2(float v) { return __int_as_float(dpp_xor2(__float_as_int(v))); }
 __device__ __forceinline__ float dppf_xor3(float v) { return __int_as_float(dpp_xor3(__float_as_int(v))); }

@@ -41,6 +41,8 @@ constexpr float MX_LOG2E = 1.4426950408889634f;
 constexpr float MX_LOW = -3.0e38f;      // below every finite score that matters; not -inf, so that differences stay numbers
 constexpr float MX_SLACK = 8.0f;
 constexpr int MX_HEADS = 8;            // query heads of a workgroup
+constexpr int MX_MAX_SPLITS = 64;      // (a lane of one wave each in the joining kernel)
+constexpr int MX_MIN_SPLIT = 256;      // keys below which a split is not worth a workgroup
 
 struct MXView {
     const unsigned char *k, *ks, *v, *vs;
@@ -55,6 +57,19 @@ struct MXPrep {                          // the step's own token (PREP instances
     int npos;
     float eps;
 };
+
+// keys of stream b (0: none, or a step that does not fit)
+template <int PREP>
+__device__ __forceinline__ int mx_length(const int* kv_len, int max_len, const MXPrep& pp, int b) {
+    const int len = kv_len[b];
+    if (!PREP) return min(len, max_len);
+    const int pos = pp.pos[b];
+    return pos < 0 || pos >= max_len || pos >= pp.npos || len != pos + 1 ? 0 : len;
+}
+// keys of a split of a stream of len: short streams use fewer of the splits
+__device__ __forceinline__ int mx_split(int len, int nsplit) {
+    return nsplit == 1 ? len : max(((len + nsplit - 1) / nsplit + 31) & ~31, MX_MIN_SPLIT);
+}
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 __device__ __forceinline__ rsrc_t mx_rsrc(const unsigned char* p, unsigned bytes) {
@@ -71,20 +86,25 @@ __device__ __forceinline__ f32x4 mx_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// A core holds T tiles of KPT keys per unit: codes k[T], v[T] (W dwords) and scale bytes ke[T], ve[T] of its lane's part of
-// each row (NP pieces, each inside one block), and the softmax state of its wave.
+// What a lane holds of a unit of T tiles: W dwords of codes of K and of V and their scale bytes
+template <int W, int T>
+struct MXUnit {
+    unsigned k[T][W], v[T][W], ke[T], ve[T];
+};
+
+// A core walks units of T tiles of KPT keys with the softmax state of its wave; its lane's part of a row consists of NP
+// pieces, each inside one block.
 
 // One query head
 template <int D, int BITS>
 struct MXOne {
     static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
     static constexpr int LR = RB / 16;                // lanes of a row
-    static constexpr int KPT = 64 / LR, T = 4, W = 4, NP = 1;
+    static constexpr int KPT = 64 / LR, T = 4, W = 4, NP = 1, NW = 4, WAVES = 4;
     static constexpr int ED = 128 / BITS;             // elements of a lane
     static constexpr int WF = BITS / 4;               // dwords of 8 elements
-    static constexpr int PARTS = 4;                   // results a wave leaves for a head: one per 16 lanes
 
-    unsigned k[T][W], v[T][W], ke[T], ve[T];
+    typedef MXUnit<W, T> Unit;
     bf16x2 q[ED / 2];
     float m, l, acc[ED], sl2;
     int lane;
@@ -110,31 +130,31 @@ struct MXOne {
 #pragma unroll
         for (int e = 0; e < ED; ++e) acc[e] = 0.f;
     }
-    __device__ __forceinline__ void load(const MXRsrc& s, int base) {
+    __device__ __forceinline__ void load(rsrc_t codes, rsrc_t scales, int base, unsigned (&c)[T][W], unsigned (&e)[T]) {
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             const int at = base + t * KPT;
-            ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at * NB + key() * NB + block(0), 0, 0);
-            ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at * NB + key() * NB + block(0), 0, 0);
-            const u32x4 x = mx_load16(s.k, at * RB + lane * 16, true), y = mx_load16(s.v, at * RB + lane * 16, true);
+            e[t] = __builtin_amdgcn_raw_buffer_load_b8(scales, at * NB + key() * NB + block(0), 0, 0);
+            const u32x4 x = mx_load16(codes, at * RB + lane * 16, true);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                k[t][i] = x[i];
-                v[t][i] = y[i];
-            }
+            for (int i = 0; i < 4; ++i) c[t][i] = x[i];
         }
     }
-    // left: keys from the unit's first on (LAST: fewer than T * KPT may be there)
+    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) {
+        load(s.k, s.ks, base, u.k, u.ke);
+        load(s.v, s.vs, base, u.v, u.ve);
+    }
+    // LAST: the unit with the split's last key, `left` keys from its first on
     template <bool LAST>
-    __device__ __forceinline__ void unit(int left) {
+    __device__ __forceinline__ void unit(const Unit& u, int left) {
         float s[T], mx = MX_LOW;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const float sc = mx_scale(ke[t]);
+            const float sc = mx_scale(u.ke[t]);
             float d[2] = {0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < ED / 8; ++j) {
-                const u32x4 x = __builtin_bit_cast(u32x4, mx_decode8<BITS>(k[t] + j * WF, sc));
+                const u32x4 x = __builtin_bit_cast(u32x4, mx_decode8<BITS>(u.k[t] + j * WF, sc));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const unsigned w = x[i];
@@ -150,9 +170,7 @@ struct MXOne {
             mx = fmaxf(mx, s[t]);
         }
         if (__any(mx > m + MX_SLACK)) {
-            float top = row16_max(mx);
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
+            const float top = fmaxf(wave64_max(mx), m);
             const float alpha = __builtin_amdgcn_exp2f(m - top);
             m = top;
             l *= alpha;
@@ -164,37 +182,52 @@ struct MXOne {
             float w = __builtin_amdgcn_exp2f(s[t] - m);
             if (LAST) w = t * KPT + key() < left ? w : 0.f;
             l += w;
-            const float sc = mx_scale(ve[t]);
+            const float sc = mx_scale(u.ve[t]);
 #pragma unroll
             for (int x = 0; x < W; ++x) {
                 constexpr int PW = 32 / BITS;
                 float f[PW];
-                mx_decode_f32<BITS>(v[t][x], sc, f);
+                mx_decode_f32<BITS>(u.v[t][x], sc, f);
 #pragma unroll
                 for (int e = 0; e < PW; ++e) acc[x * PW + e] = fmaf(w, f[e], acc[x * PW + e]);
             }
         }
     }
-    // sum over the keys of a row of 16 lanes: lanes that hold the same elements are LR apart
-    __device__ __forceinline__ static float keys_sum(float x) {
-        if (LR <= 2) x += dppf_ror2(x);
-        if (LR <= 4) x += dppf_ror4(x);
-        return x + dppf_ror8(x);
-    }
-    // maximum, denominator and sums of the wave's four rows of lanes to ml[4][2] and o[4][D]
+    // The wave's maximum, denominator and sums to ml[2] and o[D]. Lanes that hold the same elements (64 / LR keys) add up,
+    // halving the elements a lane is responsible for at every step: a swap of half waves or of neighbouring rows of 16
+    // lanes brings two elements' halves together, then exchanges inside a row.
     __device__ __forceinline__ void finish(float* ml, float* o, int nh, int hc) {
-        l = keys_sum(l);
+        l = wave64_sum(l);
+        int from = lane % LR * ED;
 #pragma unroll
-        for (int e = 0; e < ED; ++e) acc[e] = keys_sum(acc[e]);
-        const int row = lane >> 4;
-        if ((lane & 15) < LR) {
-#pragma unroll
-            for (int e = 0; e < ED; e += 4)
-                *reinterpret_cast<f32x4*>(o + row * D + (lane & 15) * ED + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+        for (int e = 0; e < ED / 2; ++e) {
+            const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[e]), __float_as_uint(acc[e + ED / 2]), false, false);
+            acc[e] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
         }
-        if ((lane & 15) == 0) {
-            ml[2 * row] = m;
-            ml[2 * row + 1] = l;
+        from += (lane >> 5 & 1) * (ED / 2);
+#pragma unroll
+        for (int e = 0; e < ED / 4; ++e) {
+            const u32x2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[e]), __float_as_uint(acc[e + ED / 4]), false, false);
+            acc[e] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        }
+        from += (lane >> 4 & 1) * (ED / 4);
+#pragma unroll
+        for (int st = 0; st < (LR == 8 ? 1 : LR == 4 ? 2 : 3); ++st) {
+            const int half = ED >> (3 + st);
+            const bool up = lane & (8 >> st);
+#pragma unroll
+            for (int e = 0; e < half; ++e) {
+                const float keep = up ? acc[e + half] : acc[e], give = up ? acc[e] : acc[e + half];
+                acc[e] = keep + (st == 0 ? dppf_ror8(give) : st == 1 ? swz_xor4(give) : dppf_xor2(give));
+            }
+            from += up ? half : 0;
+        }
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[from + e] = acc[e];
+        // the denominator: every lane of a row of the cache added the same weight
+        if (lane == 0) {
+            ml[0] = m;
+            ml[1] = l / LR;
         }
     }
 };
@@ -204,15 +237,14 @@ struct MXOne {
 template <int D, int BITS>
 struct MXHeads {
     static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
-    static constexpr int KPT = 16, T = 2, W = RB / 16;
+    static constexpr int KPT = 16, T = 2, W = RB / 16, NW = 8, WAVES = 2;
     static constexpr int NP = RB == 128 ? 2 : 1;
     static constexpr int PB = RB / 4 / NP;            // bytes of a piece
     static constexpr int PD = D / 4 / NP;             // elements of a piece
     static constexpr int NF = D / 32;                 // fragments of 8 elements
     static constexpr int WF = BITS / 4;               // dwords of a fragment
-    static constexpr int PARTS = 1;
 
-    unsigned k[T][W], v[T][W], ke[T], ve[T];          // ke, ve: one byte, or with two pieces the row's four
+    typedef MXUnit<W, T> Unit;            // (ke, ve: one byte, or with two pieces the row's four)
     bf16x8 qf[NF], pick[2];
     float m, l, sl2, low;                 // of column r; low: the column takes the weights' remainders
     f32x4 acc[NF][2];                     // rows = columns of the scores, column r of selection c
@@ -265,30 +297,28 @@ struct MXHeads {
             }
         }
     }
-    __device__ __forceinline__ void load(const MXRsrc& s, int base) {
+    __device__ __forceinline__ void load(rsrc_t codes, rsrc_t scales, int base, unsigned (&c)[T][W], unsigned (&e)[T]) {
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             const int at = base + 16 * t + r;
-            if (NP == 1) {
-                ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at * NB + block(0), 0, 0);
-                ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at * NB + block(0), 0, 0);
-            } else {
-                ke[t] = __builtin_amdgcn_raw_buffer_load_b32(s.ks, at * NB, 0, 0);
-                ve[t] = __builtin_amdgcn_raw_buffer_load_b32(s.vs, at * NB, 0, 0);
-            }
-            load_row(s.k, at * RB + g * PB, k[t]);
-            load_row(s.v, at * RB + g * PB, v[t]);
+            if (NP == 1) e[t] = __builtin_amdgcn_raw_buffer_load_b8(scales, at * NB + block(0), 0, 0);
+            else e[t] = __builtin_amdgcn_raw_buffer_load_b32(scales, at * NB, 0, 0);
+            load_row(codes, at * RB + g * PB, c[t]);
         }
     }
+    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) {
+        load(s.k, s.ks, base, u.k, u.ke);
+        load(s.v, s.vs, base, u.v, u.ve);
+    }
     template <bool LAST>
-    __device__ __forceinline__ void unit(int left) {
+    __device__ __forceinline__ void unit(const Unit& u, int left) {
         float s[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < NF; ++j)
-                a = mx_mfma(mx_decode8<BITS>(k[t] + j * WF, mx_scale(byte(ke[t], j * 8 / PD))), qf[j], a);
+                a = mx_mfma(mx_decode8<BITS>(u.k[t] + j * WF, mx_scale(byte(u.ke[t], j * 8 / PD))), qf[j], a);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[4 * t + i] = a[i] * sl2;
@@ -327,14 +357,14 @@ struct MXHeads {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int x = 0; x < NP; ++x) {
-                const unsigned e = byte(ve[t], x);
+                const unsigned e = byte(u.ve[t], x);
                 bad[x] |= __ballot(e == 255u);
                 vs[t][x] = e == 255u ? 0.f : mx_scale(e);
             }
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
-            const bf16x8 v0 = mx_decode8<BITS>(v[0] + j * WF, vs[0][j * 8 / PD]);
-            const bf16x8 v1 = mx_decode8<BITS>(v[1] + j * WF, vs[1][j * 8 / PD]);
+            const bf16x8 v0 = mx_decode8<BITS>(u.v[0] + j * WF, vs[0][j * 8 / PD]);
+            const bf16x8 v1 = mx_decode8<BITS>(u.v[1] + j * WF, vs[1][j * 8 / PD]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -375,48 +405,43 @@ struct MXHeads {
 // the new key and the new value come from the raw projection rows; the new row is quantised, takes the place of key
 // kv_len[b] - 1 in the lanes that own it, and is written to the cache by the first head group.
 template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
+__global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
                                                                  const int* __restrict__ kv_len, int H, int KVH,
                                                                  int nsplit, float scale, float* __restrict__ part_ml,
                                                                  float* __restrict__ part_o, bf16* __restrict__ out,
                                                                  long ld_o, MXPrep pp) {
     typedef Core<D, BITS> C;
-    constexpr int RB = C::RB, NB = C::NB, KPT = C::KPT, KPU = C::T * KPT, NR = NW * C::PARTS;
+    constexpr int RB = C::RB, NB = C::NB, KPT = C::KPT, KPU = C::T * KPT;
     extern __shared__ __attribute__((aligned(16))) float smem[];
 
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS;
     const int split = blockIdx.x, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
     const int h0 = kvh * group + chunk * MX_HEADS, nh = min(MX_HEADS, group - chunk * MX_HEADS), hc = min(MX_HEADS, group);
     bf16* sm_q = reinterpret_cast<bf16*>(smem);      // [hc + 2][D]: q heads, new key, new value (PREP); gives way to
-    float* sm_o = smem;                              // [NW][PARTS or heads][D] and
-    float* sm_ml = smem + NR * hc * D;               // [NW][PARTS or heads][2]
+    float* sm_o = smem;                              // [NW][hc][D] and
+    float* sm_ml = smem + NW * hc * D;               // [NW][hc][2]
     const int tid = threadIdx.x, wave = tid >> 6;
     C core;
     core.place(tid & 63);
 
-    int len = min(kv_len[b], kv.max_len);
-    const int pos = PREP ? pp.pos[b] : 0;
-    if (PREP && (pos < 0 || pos >= kv.max_len || pos >= pp.npos || kv_len[b] != pos + 1)) len = 0;
+    const int len = mx_length<PREP>(kv_len, kv.max_len, pp, b), pos = len - 1;       // (pos: of the new token, PREP)
     if (len <= 0) {                       // a stream without keys: zeros
+        if (nsplit == 1)
 #pragma unroll 1
-        for (int i = tid; i < nh * D; i += 64 * NW) {
-            const int h = h0 + i / D;
-            if (nsplit == 1) out[(long)b * ld_o + (long)h * D + i % D] = (bf16)0.f;
-            else {
-                const long pi = ((long)b * H + h) * nsplit + split;
-                part_o[pi * D + i % D] = 0.f;
-                if (i % D == 0) { part_ml[pi * 2] = 0.f; part_ml[pi * 2 + 1] = 1.f; }
-            }
-        }
+            for (int i = tid; i < nh * D; i += 64 * NW) out[(long)b * ld_o + (long)h0 * D + i] = (bf16)0.f;
         return;
     }
-    const int per = ((len + nsplit - 1) / nsplit + 31) & ~31;
+    const int per = mx_split(len, nsplit);
     const int k_beg = (int)min((long)split * per, (long)len), n = min(len - k_beg, per);     // keys of this split
+    if (n <= 0) return;
 
     const long slice = ((long)b * KVH + kvh) * kv.max_len;
     const unsigned nk = (unsigned)n;
     const MXRsrc src{mx_rsrc(kv.k + (slice + k_beg) * RB, nk * RB), mx_rsrc(kv.ks + (slice + k_beg) * NB, nk * NB),
                      mx_rsrc(kv.v + (slice + k_beg) * RB, nk * RB), mx_rsrc(kv.vs + (slice + k_beg) * NB, nk * NB)};
+
+    int base = wave * KPU;
+    typename C::Unit u;
 
     if (PREP) {
         constexpr int L16 = D / 16;
@@ -440,14 +465,13 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const bf16* __r
     }
     core.start(PREP ? sm_q : q + (long)b * ld_q + (long)h0 * D, nh, scale * MX_LOG2E);
 
-    int base = wave * KPU;
 #pragma unroll 1
     for (; base + KPU < n; base += NW * KPU) {       // units before the one with the split's last key
-        core.load(src, base);
-        core.template unit<false>(0);
+        core.load(src, base, u);
+        core.template unit<false>(u, 0);
     }
     if (base < n) {
-        core.load(src, base);
+        core.load(src, base, u);
         const int t_new = n - 1 - base;   // the stream's last key, in its last split
         if (PREP && k_beg + n == len && core.key() == t_new % KPT) {
 #pragma unroll
@@ -478,26 +502,26 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const bf16* __r
                 for (int t = 0; t < C::T; ++t)
                     if (t == t_new / KPT) {
 #pragma unroll
-                        for (int x = 0; x < C::W; ++x) (which ? core.v : core.k)[t][x] = c[x];
-                        (which ? core.ve : core.ke)[t] = all;
+                        for (int x = 0; x < C::W; ++x) (which ? u.v : u.k)[t][x] = c[x];
+                        (which ? u.ve : u.ke)[t] = all;
                     }
             }
         }
-        core.template unit<true>(n - base);
+        core.template unit<true>(u, n - base);
     }
 
     if (PREP) __syncthreads();            // sm_q lies where the sums go
-    core.finish(sm_ml + wave * C::PARTS * hc * 2, sm_o + wave * C::PARTS * hc * D, nh, hc);
+    core.finish(sm_ml + wave * hc * 2, sm_o + wave * hc * D, nh, hc);
     __syncthreads();
 #pragma unroll 1
     for (int x = tid; x < nh * D; x += 64 * NW) {
         const int i = x / D, d = x % D;
         float M = MX_LOW;
 #pragma unroll
-        for (int w = 0; w < NR; ++w) M = fmaxf(M, sm_ml[(w * hc + i) * 2]);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_ml[(w * hc + i) * 2]);
         float L = 0.f, o = 0.f;
 #pragma unroll
-        for (int w = 0; w < NR; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = __builtin_amdgcn_exp2f(sm_ml[(w * hc + i) * 2] - M);
             L += sm_ml[(w * hc + i) * 2 + 1] * f;
             o += sm_o[(w * hc + i) * D + d] * f;
@@ -514,38 +538,74 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_mx_kernel(const bf16* __r
     }
 }
 
-template <int D>
-__global__ void attn_decode_mx_merge_kernel(const float* __restrict__ part_ml, const float* __restrict__ part_o,
-                                            int nsplit, int H, bf16* __restrict__ out, long ld_o) {
-    const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
+// Joins the splits of a stream's heads: one workgroup per (head, stream), D/4 lanes per split. Latency is all that counts
+// here, so everything is requested at once, the splits that a short stream does not use among it (their memory belongs to
+// the workspace; what it holds is not looked at).
+template <int D, int PREP>
+__global__ __launch_bounds__(256) void attn_decode_mx_merge_kernel(const float* __restrict__ part_ml,
+                                                                   const float* __restrict__ part_o,
+                                                                   const int* __restrict__ kv_len, int max_len,
+                                                                   MXPrep pp, int nsplit, int H, bf16* __restrict__ out,
+                                                                   long ld_o) {
+    constexpr int L4 = D / 4, ROWS = 256 / L4, PER = MX_MAX_SPLITS / ROWS;
+    __shared__ __attribute__((aligned(16))) f32x4 sums[ROWS][L4];
+    const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x, row = t / L4, c = t % L4, lane = t & 63;
     const long p0 = ((long)b * H + h) * nsplit;
-    float M = MX_LOW;
-    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, part_ml[(p0 + s) * 2]);
-    float L = 0.f, o = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-        const float f = __builtin_amdgcn_exp2f(part_ml[(p0 + s) * 2] - M);
-        L += part_ml[(p0 + s) * 2 + 1] * f;
-        o += part_o[(p0 + s) * D + t] * f;
+    f32x4 x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (i * ROWS + row < nsplit) x[i] = *reinterpret_cast<const f32x4*>(part_o + (p0 + i * ROWS + row) * D + 4 * c);
+    float m = MX_LOW, l = 0.f;            // of split `lane`
+    if (lane < nsplit) {
+        m = part_ml[(p0 + lane) * 2];
+        l = part_ml[(p0 + lane) * 2 + 1];
     }
-    out[(long)b * ld_o + (long)h * D + t] = (bf16)(o / L);
+    const int len = mx_length<PREP>(kv_len, max_len, pp, b);
+    bf16* dst = out + (long)b * ld_o + (long)h * D;
+    if (len <= 0) {
+        if (t < D) dst[t] = (bf16)0.f;
+        return;
+    }
+    const int per = mx_split(len, nsplit), used = (len + per - 1) / per;
+    if (lane >= used) {
+        m = MX_LOW;
+        l = 0.f;
+    }
+    const float f = __builtin_amdgcn_exp2f(m - wave64_max(m)), w = f / wave64_sum(l * f);
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int s = i * ROWS + row;
+        const float ws = __shfl(w, s, 64);
+        if (s < used) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] += x[i][e] * ws;
+        }
+    }
+    sums[row][c] = a;
+    __syncthreads();
+    if (t < D) {
+        float o = 0.f;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) o += sums[i][t >> 2][t & 3];
+        dst[t] = (bf16)o;
+    }
 }
-
-constexpr int MX_MAX_SPLITS = 64;
 
 template <int D, int BITS, int PREP, template <int, int> class Core>
 void launch(const void* q, long ld_q, MXView kv, const int* kv_len, void* out, long ld_o, float* ws, int B, int H,
             int KVH, int nsplit, float scale, MXPrep pp, hipStream_t stream) {
-    constexpr int NW = 4, PARTS = Core<D, BITS>::PARTS;
+    constexpr int NW = Core<D, BITS>::NW;
     float* part_ml = ws;
     float* part_o = ws ? ws + (long)B * H * nsplit * 2 : nullptr;
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS, hc = group < MX_HEADS ? group : MX_HEADS;
-    const int lds = NW * PARTS * hc * (D + 2) * 4;   // (more than the PREP rows: (hc + 2) * D * 2 bytes)
+    const int lds = NW * hc * (D + 2) * 4;           // (more than the PREP rows: (hc + 2) * D * 2 bytes)
     hipLaunchKernelGGL((attn_decode_mx_kernel<D, BITS, PREP, Core, NW>), dim3(nsplit, KVH * chunks, B), dim3(64 * NW), lds,
                        stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, scale, part_ml, part_o, (bf16*)out, ld_o,
                        pp);
     if (nsplit > 1)
-        hipLaunchKernelGGL((attn_decode_mx_merge_kernel<D>), dim3(H, B), dim3(D), 0, stream, part_ml, part_o, nsplit, H,
-                           (bf16*)out, ld_o);
+        hipLaunchKernelGGL((attn_decode_mx_merge_kernel<D, PREP>), dim3(H, B), dim3(256), 0, stream, part_ml, part_o, kv_len,
+                           kv.max_len, pp, nsplit, H, (bf16*)out, ld_o);
 }
 
 template <int PREP>
@@ -578,14 +638,29 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 
 }  // namespace
 
-// Key splits for a call whose longest stream has `longest` keys
+// Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
+// Few workgroups (below): as many splits as bring them to 512, each with keys for two rounds of its waves or more, where
+// the second launch is worth its 3 us: from 8 rounds on (1 stream x 8 heads x 128 in 8 bits: 4096 keys, 32 rounds, 24.5 us
+// in one split and 9.0 in 16; 512 keys, 4 rounds, 5.4 and 7.2).
+// Many: one, unless that leaves the last round of the chip's 1024 places less than 7/8 full (64 streams x 24 heads x 2047
+// keys: 1536 workgroups, 79 us in one split and 70 in two; 256 x 8: 166 and 172).
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
     if (B <= 0 || KVH <= 0 || H < KVH || longest <= 0) return 1;
-    const int chunks = (H / KVH + MX_HEADS - 1) / MX_HEADS;
-    const long groups = (long)B * KVH * chunks;
-    const long want = (1024 + groups - 1) / groups, most = (longest + 255) / 256;
-    const long n = groups >= 1024 ? 1 : want < most ? want : most;
-    return (int)(n < 1 ? 1 : n > MX_MAX_SPLITS ? MX_MAX_SPLITS : n);
+    const long groups = (long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS);
+    // keys of one round of a workgroup's waves, taken at 8 bits
+    const int round = H == KVH ? (D == 128 ? 128 : 256) : 256;
+    const int rounds = (longest + round - 1) / round;
+    if (rounds < 8) return 1;
+    if (groups < 256) {
+        const long n = 512 / groups, most = rounds / 2;
+        return (int)(n < most ? (n < MX_MAX_SPLITS ? n : MX_MAX_SPLITS) : most < MX_MAX_SPLITS ? most : MX_MAX_SPLITS);
+    }
+    if (groups > 1024)
+        for (int n = 1; n <= 4; ++n) {
+            const long wg = groups * n, places = (wg + 1023) / 1024 * 1024;
+            if (8 * wg >= 7 * places) return n;
+        }
+    return 1;
 }
 
 // q [B][ld_q] (heads at h*D), out [B][ld_o] bf16; kv_len[b] = cached keys of stream b (0: the output row is zeros; values

@@ -106,17 +106,15 @@ __device__ __forceinline__ void mx_decode_f32(unsigned c, float s, float* out) {
 // exchanges inside a row of 16 lanes (no LDS traffic): lane i gets the value of lane ...
 __device__ __forceinline__ int dpp_xor1(int v) { return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true); }
 __device__ __forceinline__ int dpp_xor2(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true); }
-__device__ __forceinline__ int dpp_xor3(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x1B, 0xF, 0xF, true); }
 __device__ __forceinline__ int dpp_xor7(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true); }   // 7 - i in 8
 __device__ __forceinline__ int dpp_xor15(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true); }  // 15 - i
-__device__ __forceinline__ float dppf_ror2(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xF, 0xF, true)); }
-__device__ __forceinline__ float dppf_ror4(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xF, 0xF, true)); }
 __device__ __forceinline__ float dppf_ror8(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true)); }
 __device__ __forceinline__ float dppf_xor1(float v) { return __int_as_float(dpp_xor1(__float_as_int(v))); }
 __device__ __forceinline__ float dppf_xor2(float v) { return __int_as_float(dpp_xor2(__float_as_int(v))); }
-__device__ __forceinline__ float dppf_xor3(float v) { return __int_as_float(dpp_xor3(__float_as_int(v))); }
 __device__ __forceinline__ float dppf_xor7(float v) { return __int_as_float(dpp_xor7(__float_as_int(v))); }
 __device__ __forceinline__ float dppf_xor15(float v) { return __int_as_float(dpp_xor15(__float_as_int(v))); }
+
+__device__ __forceinline__ float swz_xor4(float v) { return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 4 << 10 | 0x1F)); }
 
 // sum / maximum over a row of 16 lanes, in every lane of it
 __device__ __forceinline__ float row16_sum(float v) {
@@ -130,4 +128,15 @@ __device__ __forceinline__ float row16_max(float v) {
     v = fmaxf(v, dppf_xor2(v));
     v = fmaxf(v, dppf_xor7(v));
     return fmaxf(v, dppf_xor15(v));
+}
+// over the wave
+__device__ __forceinline__ float wave64_sum(float v) {
+    v = row16_sum(v);
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+__device__ __forceinline__ float wave64_max(float v) {
+    v = row16_max(v);
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
 }

@@ -623,6 +623,7 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
     MGEN_REQUIRE(nsplit == 1 || ws != nullptr, "%s: nsplit > 1 needs a workspace", what);
     MGEN_REQUIRE(ld_o >= (long)H * D, "%s: output rows overlap (ld_o below H * D)", what);
     MGEN_REQUIRE((((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, "%s: codes must be 16-byte aligned", what);
+    MGEN_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (D / 32 - 1)) == 0, "%s: scales must be aligned to a row (D / 32)", what);
     const MXView kv{(const unsigned char*)kc, (const unsigned char*)ks, (const unsigned char*)vc,
                     (const unsigned char*)vs, max_len};
 #define LAUNCH(DD, BB)                                                                                                 \

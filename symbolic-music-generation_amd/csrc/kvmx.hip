@@ -17,27 +17,32 @@ inline FastDiv fast_div(unsigned d) {
 }
 __device__ __forceinline__ unsigned fdiv(unsigned n, FastDiv f) { return (__umulhi(n, f.m) + n) >> f.s; }
 
-struct MXRows {                 // the rows of one call, numbered with the token index innermost
-    FastDiv tokens, heads;
-    unsigned nrows;
+// The rows of one call, numbered tile by tile: up to a workgroup's worth of consecutive tokens of one head, then the next
+// head, then the next tokens. A tile's cache rows are one contiguous run; neighbouring workgroups take the heads of the
+// same tokens, so that the chip reads (writes) whole token rows at a time. (All tokens of a head first, as the cache lies,
+// put every workgroup on the same 256-byte column of rows whose pitch is a multiple of the memory channels' period.)
+struct MXRows {
+    FastDiv tiles, heads;
+    unsigned nrows, tokens;
+    int shift;                  // tile = 1 << shift tokens
     int max_len;
     const int* pos0;
 };
 
 struct Row {
     bool there;
-    long src, slot;             // element offset of the head in the token-major rows / row index in the cache
+    long tok, head, slot;       // row of the token-major side, head in it, row of the cache
 };
 
-__device__ __forceinline__ Row locate(const MXRows& a, unsigned row, long ld, int D) {
-    const unsigned t = fdiv(row, a.tokens), i = row - t * a.tokens.d;
-    const unsigned b = fdiv(t, a.heads), h = t - b * a.heads.d;
+__device__ __forceinline__ Row locate(const MXRows& a, unsigned row) {
+    const unsigned x = row >> a.shift, t = fdiv(x, a.heads), h = x - t * a.heads.d, b = fdiv(t, a.tiles);
+    const unsigned i = ((t - b * a.tiles.d) << a.shift) + (row & ((1u << a.shift) - 1));
+    if (row >= a.nrows || i >= a.tokens) return {false, 0, 0, 0};
     const int p = (int)((unsigned)a.pos0[b] + i);
-    return {p >= 0 && p < a.max_len, ((long)b * a.tokens.d + i) * ld + (long)h * D,
-            ((long)b * a.heads.d + h) * a.max_len + p};
+    return {p >= 0 && p < a.max_len, (long)b * a.tokens + i, (long)h, ((long)b * a.heads.d + h) * a.max_len + p};
 }
 
-// D/8 lanes per row, 8 elements per lane; a block is 4 lanes
+// D/8 lanes per row of K and of V, 8 elements per lane; a block is 4 lanes
 template <int D, int BITS>
 __global__ __launch_bounds__(256) void kv_append_mx_kernel(const bf16* __restrict__ k_src, const bf16* __restrict__ v_src,
                                                            long ld_k, long ld_v, unsigned char* __restrict__ kc,
@@ -46,22 +51,23 @@ __global__ __launch_bounds__(256) void kv_append_mx_kernel(const bf16* __restric
                                                            unsigned char* __restrict__ vs, MXRows a) {
     constexpr int LPR = D / 8, RPB = 256 / LPR, RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
     const int sub = threadIdx.x % LPR;
-    const unsigned row = blockIdx.x * RPB + threadIdx.x / LPR;
-    if (row >= a.nrows) return;
-    const bool is_v = blockIdx.y != 0;
-    const Row w = locate(a, row, is_v ? ld_v : ld_k, D);
+    const Row w = locate(a, blockIdx.x * RPB + threadIdx.x / LPR);
     if (!w.there) return;       // the lanes of a row leave together
-    const bf16x8 x = *reinterpret_cast<const bf16x8*>((is_v ? v_src : k_src) + w.src + sub * 8);
-    unsigned top = mx_top8(x);
-    top = max(top, (unsigned)dpp_xor1((int)top));
-    top = max(top, (unsigned)dpp_xor2((int)top));
-    const unsigned e = mx_exponent<BITS>(top);
-    unsigned c[2];
-    mx_encode8<BITS>(x, e, c);
-    unsigned char* codes = (is_v ? vc : kc) + w.slot * RB + sub * BITS;
-    if (BITS == 4) *reinterpret_cast<unsigned*>(codes) = c[0];
-    else *reinterpret_cast<u32x2*>(codes) = u32x2{c[0], c[1]};
-    if ((sub & 3) == 0) (is_v ? vs : ks)[w.slot * NB + (sub >> 2)] = (unsigned char)e;
+    const bf16x8 x[2] = {*reinterpret_cast<const bf16x8*>(k_src + w.tok * ld_k + w.head * D + sub * 8),
+                         *reinterpret_cast<const bf16x8*>(v_src + w.tok * ld_v + w.head * D + sub * 8)};
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        unsigned top = mx_top8(x[which]);
+        top = max(top, (unsigned)dpp_xor1((int)top));
+        top = max(top, (unsigned)dpp_xor2((int)top));
+        const unsigned e = mx_exponent<BITS>(top);
+        unsigned c[2];
+        mx_encode8<BITS>(x[which], e, c);
+        unsigned char* codes = (which ? vc : kc) + w.slot * RB + sub * BITS;
+        if (BITS == 4) *reinterpret_cast<unsigned*>(codes) = c[0];
+        else *reinterpret_cast<u32x2*>(codes) = u32x2{c[0], c[1]};
+        if ((sub & 3) == 0) (which ? vs : ks)[w.slot * NB + (sub >> 2)] = (unsigned char)e;
+    }
 }
 
 template <int D, int BITS>
@@ -72,21 +78,24 @@ __global__ __launch_bounds__(256) void kv_read_mx_kernel(const unsigned char* __
                                                          bf16* __restrict__ v_dst, long ld_k, long ld_v, MXRows a) {
     constexpr int LPR = D / 8, RPB = 256 / LPR, RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
     const int sub = threadIdx.x % LPR;
-    const unsigned row = blockIdx.x * RPB + threadIdx.x / LPR;
-    if (row >= a.nrows) return;
-    const bool is_v = blockIdx.y != 0;
-    const Row w = locate(a, row, is_v ? ld_v : ld_k, D);
+    const Row w = locate(a, blockIdx.x * RPB + threadIdx.x / LPR);
     if (!w.there) return;
-    const unsigned char* codes = (is_v ? vc : kc) + w.slot * RB + sub * BITS;
-    unsigned c[2];
-    if (BITS == 4) c[0] = *reinterpret_cast<const unsigned*>(codes);
-    else {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(codes);
-        c[0] = v[0];
-        c[1] = v[1];
+    unsigned c[2][2], e[2];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        const unsigned char* codes = (which ? vc : kc) + w.slot * RB + sub * BITS;
+        if (BITS == 4) c[which][0] = *reinterpret_cast<const unsigned*>(codes);
+        else {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(codes);
+            c[which][0] = v[0];
+            c[which][1] = v[1];
+        }
+        e[which] = (which ? vs : ks)[w.slot * NB + (sub >> 2)];
     }
-    const float s = mx_scale((is_v ? vs : ks)[w.slot * NB + (sub >> 2)]);
-    *reinterpret_cast<bf16x8*>((is_v ? v_dst : k_dst) + w.src + sub * 8) = mx_decode8<BITS>(c, s);
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+        st_stream(reinterpret_cast<bf16x8*>((which ? v_dst : k_dst) + w.tok * (which ? ld_v : ld_k) + w.head * D + sub * 8),
+                  mx_decode8<BITS>(c[which], mx_scale(e[which])));
 }
 
 // what the two calls check alike; fills the row numbering
@@ -102,8 +111,12 @@ int rows_of(const char* what, const void* k, const void* v, const void* kc, cons
     MGEN_REQUIRE(ld_k >= (long)KVH * D && ld_v >= (long)KVH * D, "%s: rows overlap (stride below KVH * D)", what);
     MGEN_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0,
                  "%s: rows and codes must be 16-byte aligned", what);
-    MGEN_REQUIRE((long)B * n * KVH < (1l << 31), "%s: too many rows", what);
-    *a = {fast_div((unsigned)n), fast_div((unsigned)KVH), (unsigned)((long)B * n * KVH), max_len, pos0};
+    MGEN_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (D / 32 - 1)) == 0, "%s: scales must be aligned to a row (D / 32)", what);
+    int shift = 0;              // a tile: at most the rows of a workgroup, no more than the tokens need
+    while ((1 << shift) < 2048 / D && (1 << shift) < n) ++shift;
+    const long tiles = ((long)n + (1 << shift) - 1) >> shift, rows = (B * tiles * KVH) << shift;
+    MGEN_REQUIRE(rows < (1l << 31), "%s: too many rows (%ld)", what, rows);
+    *a = {fast_div((unsigned)tiles), fast_div((unsigned)KVH), (unsigned)rows, (unsigned)n, shift, max_len, pos0};
     return MGEN_OK;
 }
 
@@ -125,7 +138,7 @@ extern "C" int mgen_kv_append_mx(const void* k_src, const void* v_src, long ld_k
                         n_new, KVH, D, max_len, bits, &a))
         return e;
 #define LAUNCH(DD, BB)                                                                                               \
-    hipLaunchKernelGGL((kv_append_mx_kernel<DD, BB>), dim3((a.nrows + 2048 / DD - 1) / (2048 / DD), 2), dim3(256), 0, \
+    hipLaunchKernelGGL((kv_append_mx_kernel<DD, BB>), dim3((a.nrows + 2048 / DD - 1) / (2048 / DD)), dim3(256), 0,    \
                        stream, (const bf16*)k_src, (const bf16*)v_src, ld_k, ld_v, (unsigned char*)k_codes,          \
                        (unsigned char*)k_scales, (unsigned char*)v_codes, (unsigned char*)v_scales, a)
     MX_DISPATCH(LAUNCH);
@@ -143,7 +156,7 @@ extern "C" int mgen_kv_read_mx(const void* k_codes, const void* k_scales, const 
                         KVH, D, max_len, bits, &a))
         return e;
 #define LAUNCH(DD, BB)                                                                                               \
-    hipLaunchKernelGGL((kv_read_mx_kernel<DD, BB>), dim3((a.nrows + 2048 / DD - 1) / (2048 / DD), 2), dim3(256), 0,   \
+    hipLaunchKernelGGL((kv_read_mx_kernel<DD, BB>), dim3((a.nrows + 2048 / DD - 1) / (2048 / DD)), dim3(256), 0,      \
                        stream, (const unsigned char*)k_codes, (const unsigned char*)k_scales,                        \
                        (const unsigned char*)v_codes, (const unsigned char*)v_scales, (bf16*)k_dst, (bf16*)v_dst,    \
                        ld_k, ld_v, a)

@@ -636,8 +636,8 @@ class MXKV:
                              f"{k_scale.shape[3]} scales a row")
         if len({t.device for t in (k, k_scale, v, v_scale)}) != 1:
             raise ValueError("the parts of a quantised cache must be on one device")
-        if k.data_ptr() % 16 or v.data_ptr() % 16:
-            raise ValueError("the codes of a quantised cache must be 16-byte aligned")
+        if k.data_ptr() % 16 or v.data_ptr() % 16 or k_scale.data_ptr() % (self.D // 32) or v_scale.data_ptr() % (self.D // 32):
+            raise ValueError("a quantised cache's codes must be 16-byte aligned, its scales to a row (D / 32 bytes)")
         _need_gpu(k)
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
         self.fmt = "mxfp4" if self.bits == 4 else "mxfp8"
@@ -656,14 +656,14 @@ class MXKV:
         """Streams [b0, b1) (views)."""
         return MXKV(self.k[b0:b1], self.k_scale[b0:b1], self.v[b0:b1], self.v_scale[b0:b1])
 
-    def _check(self, B, **per_stream):
+    def _check(self, B, name, t):
+        """B streams with their int32 tensor `t`, on the current device."""
         if not 0 < B <= self.B:
             raise ValueError(f"{B} streams, the cache holds {self.B}")
         if self.device.index != torch.cuda.current_device():
             raise RuntimeError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        for name, t in per_stream.items():
-            if t.dtype != torch.int32 or t.numel() < B or not t.is_contiguous() or t.device != self.device:
-                raise ValueError(f"{name} must be a contiguous int32 tensor of {B} entries on {self.device}")
+        if t.dtype is not torch.int32 or t.numel() < B or not t.is_contiguous() or t.device != self.device:
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {B} entries on {self.device}")
 
     def _rows(self, x, name, n, ld, width):
         """Address of [n][ld] bf16 rows of which `width` elements are used: a raw device pointer (int) as it is, a
@@ -672,18 +672,19 @@ class MXKV:
             raise ValueError(f"{name}: a row stride of {ld} for rows of {width} elements")
         if isinstance(x, int):
             return x
-        if x.dtype != torch.bfloat16 or x.device != self.device or x.dim() != 2 or x.stride(1) != 1:
+        shape, strides = x.shape, x.stride()
+        if x.dtype is not torch.bfloat16 or x.device != self.device or len(shape) != 2 or strides[1] != 1:
             raise ValueError(f"{name} must be a 2-dimensional bfloat16 tensor on {self.device} with unit element stride")
-        if x.shape[0] < n or x.shape[1] < width or (n > 1 and x.stride(0) != ld):
+        if shape[0] < n or shape[1] < width or (n > 1 and strides[0] != ld):
             raise ValueError(f"{name}: {n} rows of {width} elements with stride {ld} from a tensor of shape "
-                             f"{tuple(x.shape)} with stride {x.stride(0)}")
+                             f"{tuple(shape)} with stride {strides[0]}")
         return x.data_ptr()
 
 
 def kv_append_mx(k_src, v_src, ld_k, ld_v, kv, pos0, B, n_new):
     """kv_append into a quantised cache: rows k_src/v_src [B*n_new][ld] bf16 (tensors or raw device pointers) into slots
     pos0[b] .. pos0[b] + n_new - 1 of stream b; slots outside the cache are skipped."""
-    kv._check(B, pos0=pos0)
+    kv._check(B, "pos0", pos0)
     w = kv.KVH * kv.D
     call("mgen_kv_append_mx", kv._rows(k_src, "k_src", B * n_new, ld_k, w), kv._rows(v_src, "v_src", B * n_new, ld_v, w),
          ld_k, ld_v, *kv.ptrs, pos0.data_ptr(), B, n_new, kv.KVH, kv.D, kv.max_len, kv.bits, _stream())
@@ -692,7 +693,7 @@ def kv_append_mx(k_src, v_src, ld_k, ld_v, kv, pos0, B, n_new):
 def kv_read_mx(kv, pos0, k_dst, v_dst, ld_k, ld_v, B, n):
     """The inverse of kv_append_mx: the values of slots pos0[b] .. pos0[b] + n - 1 into rows k_dst/v_dst [B*n][ld] bf16;
     rows whose slot is outside the cache stay as they were."""
-    kv._check(B, pos0=pos0)
+    kv._check(B, "pos0", pos0)
     w = kv.KVH * kv.D
     call("mgen_kv_read_mx", *kv.ptrs, pos0.data_ptr(), kv._rows(k_dst, "k_dst", B * n, ld_k, w),
          kv._rows(v_dst, "v_dst", B * n, ld_v, w), ld_k, ld_v, B, n, kv.KVH, kv.D, kv.max_len, kv.bits, _stream())
@@ -707,16 +708,16 @@ def _mx_workspace(workspace, B, H, D, nsplit):
     if nsplit > 1:
         if workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous() or not workspace.is_cuda:
             raise ValueError("nsplit > 1 needs a contiguous fp32 workspace on the GPU")
-        if workspace.numel() < attn_decode_workspace(B, H, D, nsplit):
-            raise ValueError(f"a workspace of {workspace.numel()} floats, attn_decode_workspace asks for "
-                             f"{attn_decode_workspace(B, H, D, nsplit)}")
+        need = _lib.lib().mgen_attn_decode_workspace(B, H, D, nsplit)
+        if workspace.numel() < need:
+            raise ValueError(f"a workspace of {workspace.numel()} floats, attn_decode_workspace asks for {need}")
     return _p(workspace)
 
 
 def attn_decode_mx(q, ld_q, kv, kv_len, out, ld_o, workspace, B, H, nsplit, scale):
     """attn_decode over a quantised cache (an MXKV). q/out: rows [B][ld] bf16 (tensors or raw device pointers); a stream
     with kv_len[b] = 0 gets zeros, kv_len[b] beyond the cache counts as the cache's length."""
-    kv._check(B, kv_len=kv_len)
+    kv._check(B, "kv_len", kv_len)
     D = kv.D
     call("mgen_attn_decode_mx", kv._rows(q, "q", B, ld_q, H * D), ld_q, *kv.ptrs, kv_len.data_ptr(),
          kv._rows(out, "out", B, ld_o, H * D), ld_o, _mx_workspace(workspace, B, H, D, nsplit), B, H, kv.KVH, D,
@@ -728,7 +729,8 @@ def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_le
     """attn_decode_prep over a quantised cache (an MXKV): q, new key and value from the raw projection rows, the new row
     quantised into slot pos[b] and attended. A stream whose pos[b] is no row of the cache or of the rotary table cs, or
     whose kv_len[b] is not pos[b] + 1, gets zeros and is not written."""
-    kv._check(B, pos=pos, kv_len=kv_len)
+    kv._check(B, "pos", pos)
+    kv._check(B, "kv_len", kv_len)
     D = kv.D
     for t, n, name in ((wq, D, "wq"), (wk, D, "wk"), (cs, D, "cs")):
         if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.device != kv.device or t.numel() < n):
@@ -741,7 +743,8 @@ def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_le
 def decode_layer_mx(ptrs17, cs, pos, kv_len, kv, B, d, H, I, nsplit, eps, interleaved):
     """decode_layer over a quantised cache (an MXKV): ptrs17 as there; cs is the rotary table [positions, D/2, 2], pos and
     kv_len int32 tensors of at least B entries."""
-    kv._check(B, pos=pos, kv_len=kv_len)
+    kv._check(B, "pos", pos)
+    kv._check(B, "kv_len", kv_len)
     call("mgen_decode_layer_mx", *ptrs17, _p(cs), cs.shape[0], _p(pos), _p(kv_len), *kv.ptrs, B, d, H, kv.KVH, kv.D, I,
          kv.max_len, kv.bits, nsplit, eps, interleaved, _stream())
 

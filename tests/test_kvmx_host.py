@@ -35,10 +35,11 @@ def _prep(**kw):
 
 ROWS = [dict(k=None), dict(v=None), dict(kc=None), dict(ks=None), dict(vc=None), dict(vs=None), dict(pos=None), dict(B=0),
         dict(n=0), dict(n=-1), dict(KVH=0), dict(D=96), dict(D=32), dict(L=0), dict(bits=6), dict(ldk=1020), dict(ldv=1023),
-        dict(ldk=512), dict(k=4104), dict(v=4098), dict(kc=4100), dict(vc=4104), dict(B=70000, n=70000)]
+        dict(ldk=512), dict(k=4104), dict(v=4098), dict(kc=4100), dict(vc=4104), dict(B=70000, n=70000), dict(ks=4098), dict(vs=4097), dict(D=64, ks=4097)]
 ATTN = [dict(kc=None), dict(ks=None), dict(vc=None), dict(vs=None), dict(n=None), dict(out=None), dict(B=0), dict(B=65536),
         dict(H=0), dict(KVH=0), dict(H=9, KVH=2, ldo=4096), dict(D=256), dict(L=0), dict(L=1 << 24), dict(bits=16),
-        dict(split=0), dict(split=65), dict(split=2, ws=None), dict(ldo=1000), dict(kc=4104), dict(vc=4097),
+        dict(split=0), dict(split=65), dict(split=2, ws=None), dict(ldo=1000), dict(kc=4104), dict(vc=4097), dict(ks=4098),
+        dict(vs=4097), dict(D=64, vs=4097),
         dict(H=65536, KVH=65536, ldo=1 << 24)]
 
 

@@ -100,7 +100,9 @@ template <int D, int BITS>
 struct MXOne {
     static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
     static constexpr int LR = RB / 16;                // lanes of a row
-    static constexpr int KPT = 64 / LR, T = 4, W = 4, NP = 1, NW = 4, WAVES = 4;
+    static constexpr int KPT = 64 / LR, T = 4, W = 4, NP = 1, NW = 4;
+    // waves a SIMD has to hold; the step's instances in 4 bits would spill at the 128 registers that 4 waves leave
+    static constexpr int waves(int prep) { return BITS == 4 && prep ? 3 : 4; }
     static constexpr int ED = 128 / BITS;             // elements of a lane
     static constexpr int WF = BITS / 4;               // dwords of 8 elements
 
@@ -237,7 +239,8 @@ struct MXOne {
 template <int D, int BITS>
 struct MXHeads {
     static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
-    static constexpr int KPT = 16, T = 2, W = RB / 16, NW = 8, WAVES = 2;
+    static constexpr int KPT = 16, T = 2, W = RB / 16, NW = 8;
+    static constexpr int waves(int) { return 2; }
     static constexpr int NP = RB == 128 ? 2 : 1;
     static constexpr int PB = RB / 4 / NP;            // bytes of a piece
     static constexpr int PD = D / 4 / NP;             // elements of a piece
@@ -405,7 +408,7 @@ struct MXHeads {
 // the new key and the new value come from the raw projection rows; the new row is quantised, takes the place of key
 // kv_len[b] - 1 in the lanes that own it, and is written to the cache by the first head group.
 template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
-__global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
+__global__ __launch_bounds__(64 * NW, (Core<D, BITS>::waves(PREP))) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
                                                                  const int* __restrict__ kv_len, int H, int KVH,
                                                                  int nsplit, float scale, float* __restrict__ part_ml,
                                                                  float* __restrict__ part_o, bf16* __restrict__ out,
@@ -640,9 +643,9 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 }  // namespace
 
 // Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
-// Few workgroups (below): as many splits as bring them to 512, each with keys for two rounds of its waves or more, where
-// the second launch is worth its 3 us: from 8 rounds on (1 stream x 8 heads x 128 in 8 bits: 4096 keys, 32 rounds, 24.5 us
-// in one split and 9.0 in 16; 512 keys, 4 rounds, 5.4 and 7.2).
+// Few workgroups: as many splits as bring them to 512, each with keys for two rounds of its waves (several heads: one) or
+// more, where the second launch is worth its 3 us: from 8 rounds on (1 stream x 8 heads x 128 in 8 bits: 4096 keys, 32
+// rounds, 24.5 us in one split and 7.4 in 16; 512 keys, 4 rounds, 5.4 and 7.2).
 // Many: one, unless that leaves the last round of the chip's 1024 places less than 7/8 full (64 streams x 24 heads x 2047
 // keys: 1536 workgroups, 79 us in one split and 70 in two; 256 x 8: 166 and 172).
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
@@ -653,7 +656,7 @@ extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int long
     const int rounds = (longest + round - 1) / round;
     if (rounds < 8) return 1;
     if (groups < 256) {
-        const long n = 512 / groups, most = rounds / 2;
+        const long n = 512 / groups, most = H == KVH ? rounds / 2 : rounds;
         return (int)(n < most ? (n < MX_MAX_SPLITS ? n : MX_MAX_SPLITS) : most < MX_MAX_SPLITS ? most : MX_MAX_SPLITS);
     }
     if (groups > 1024)

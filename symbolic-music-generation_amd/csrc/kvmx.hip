@@ -37,7 +37,7 @@ struct Row {
 __device__ __forceinline__ Row locate(const MXRows& a, unsigned row) {
     const unsigned x = row >> a.shift, t = fdiv(x, a.heads), h = x - t * a.heads.d, b = fdiv(t, a.tiles);
     const unsigned i = ((t - b * a.tiles.d) << a.shift) + (row & ((1u << a.shift) - 1));
-    if (row >= a.nrows || i >= a.tokens) return {false, 0, 0, 0};
+    if (i >= a.tokens) return {false, 0, 0, 0};
     const int p = (int)((unsigned)a.pos0[b] + i);
     return {p >= 0 && p < a.max_len, (long)b * a.tokens + i, (long)h, ((long)b * a.heads.d + h) * a.max_len + p};
 }
@@ -51,22 +51,24 @@ __global__ __launch_bounds__(256) void kv_append_mx_kernel(const bf16* __restric
                                                            unsigned char* __restrict__ vs, MXRows a) {
     constexpr int LPR = D / 8, RPB = 256 / LPR, RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
     const int sub = threadIdx.x % LPR;
-    const Row w = locate(a, blockIdx.x * RPB + threadIdx.x / LPR);
-    if (!w.there) return;       // the lanes of a row leave together
-    const bf16x8 x[2] = {*reinterpret_cast<const bf16x8*>(k_src + w.tok * ld_k + w.head * D + sub * 8),
-                         *reinterpret_cast<const bf16x8*>(v_src + w.tok * ld_v + w.head * D + sub * 8)};
+    for (unsigned row = blockIdx.x * RPB + threadIdx.x / LPR; row < a.nrows; row += gridDim.x * RPB) {
+        const Row w = locate(a, row);
+        if (!w.there) continue;                 // (all lanes of a row alike)
+        const bf16x8 x[2] = {*reinterpret_cast<const bf16x8*>(k_src + w.tok * ld_k + w.head * D + sub * 8),
+                             *reinterpret_cast<const bf16x8*>(v_src + w.tok * ld_v + w.head * D + sub * 8)};
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        unsigned top = mx_top8(x[which]);
-        top = max(top, (unsigned)dpp_xor1((int)top));
-        top = max(top, (unsigned)dpp_xor2((int)top));
-        const unsigned e = mx_exponent<BITS>(top);
-        unsigned c[2];
-        mx_encode8<BITS>(x[which], e, c);
-        unsigned char* codes = (which ? vc : kc) + w.slot * RB + sub * BITS;
-        if (BITS == 4) *reinterpret_cast<unsigned*>(codes) = c[0];
-        else *reinterpret_cast<u32x2*>(codes) = u32x2{c[0], c[1]};
-        if ((sub & 3) == 0) (which ? vs : ks)[w.slot * NB + (sub >> 2)] = (unsigned char)e;
+        for (int which = 0; which < 2; ++which) {
+            unsigned top = mx_top8(x[which]);
+            top = max(top, (unsigned)dpp_xor1((int)top));
+            top = max(top, (unsigned)dpp_xor2((int)top));
+            const unsigned e = mx_exponent<BITS>(top);
+            unsigned c[2];
+            mx_encode8<BITS>(x[which], e, c);
+            unsigned char* codes = (which ? vc : kc) + w.slot * RB + sub * BITS;
+            if (BITS == 4) *reinterpret_cast<unsigned*>(codes) = c[0];
+            else *reinterpret_cast<u32x2*>(codes) = u32x2{c[0], c[1]};
+            if ((sub & 3) == 0) (which ? vs : ks)[w.slot * NB + (sub >> 2)] = (unsigned char)e;
+        }
     }
 }
 
@@ -78,24 +80,33 @@ __global__ __launch_bounds__(256) void kv_read_mx_kernel(const unsigned char* __
                                                          bf16* __restrict__ v_dst, long ld_k, long ld_v, MXRows a) {
     constexpr int LPR = D / 8, RPB = 256 / LPR, RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
     const int sub = threadIdx.x % LPR;
-    const Row w = locate(a, blockIdx.x * RPB + threadIdx.x / LPR);
-    if (!w.there) return;
-    unsigned c[2][2], e[2];
+    for (unsigned row = blockIdx.x * RPB + threadIdx.x / LPR; row < a.nrows; row += gridDim.x * RPB) {
+        const Row w = locate(a, row);
+        if (!w.there) continue;
+        unsigned c[2][2], e[2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const unsigned char* codes = (which ? vc : kc) + w.slot * RB + sub * BITS;
-        if (BITS == 4) c[which][0] = *reinterpret_cast<const unsigned*>(codes);
-        else {
-            const u32x2 v = *reinterpret_cast<const u32x2*>(codes);
-            c[which][0] = v[0];
-            c[which][1] = v[1];
+        for (int which = 0; which < 2; ++which) {
+            const unsigned char* codes = (which ? vc : kc) + w.slot * RB + sub * BITS;
+            if (BITS == 4) c[which][0] = *reinterpret_cast<const unsigned*>(codes);
+            else {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(codes);
+                c[which][0] = v[0];
+                c[which][1] = v[1];
+            }
+            e[which] = (which ? vs : ks)[w.slot * NB + (sub >> 2)];
         }
-        e[which] = (which ? vs : ks)[w.slot * NB + (sub >> 2)];
-    }
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
-        st_stream(reinterpret_cast<bf16x8*>((which ? v_dst : k_dst) + w.tok * (which ? ld_v : ld_k) + w.head * D + sub * 8),
-                  mx_decode8<BITS>(c[which], mx_scale(e[which])));
+        for (int which = 0; which < 2; ++which)
+            st_stream(reinterpret_cast<bf16x8*>((which ? v_dst : k_dst) + w.tok * (which ? ld_v : ld_k) + w.head * D + sub * 8),
+                      mx_decode8<BITS>(c[which], mx_scale(e[which])));
+    }
+}
+
+// workgroups of 256 threads for the rows of a call (more rows than 2^20 of them hold: a workgroup takes several)
+template <int D>
+unsigned blocks_for(unsigned rows) {
+    const unsigned n = (rows + 2048 / D - 1) / (2048 / D);
+    return n < 1u << 20 ? n : 1u << 20;
 }
 
 // what the two calls check alike; fills the row numbering
@@ -138,7 +149,7 @@ extern "C" int mgen_kv_append_mx(const void* k_src, const void* v_src, long ld_k
                         n_new, KVH, D, max_len, bits, &a))
         return e;
 #define LAUNCH(DD, BB)                                                                                               \
-    hipLaunchKernelGGL((kv_append_mx_kernel<DD, BB>), dim3((a.nrows + 2048 / DD - 1) / (2048 / DD)), dim3(256), 0,    \
+    hipLaunchKernelGGL((kv_append_mx_kernel<DD, BB>), dim3(blocks_for<DD>(a.nrows)), dim3(256), 0,                    \
                        stream, (const bf16*)k_src, (const bf16*)v_src, ld_k, ld_v, (unsigned char*)k_codes,          \
                        (unsigned char*)k_scales, (unsigned char*)v_codes, (unsigned char*)v_scales, a)
     MX_DISPATCH(LAUNCH);
@@ -156,7 +167,7 @@ extern "C" int mgen_kv_read_mx(const void* k_codes, const void* k_scales, const 
                         KVH, D, max_len, bits, &a))
         return e;
 #define LAUNCH(DD, BB)                                                                                               \
-    hipLaunchKernelGGL((kv_read_mx_kernel<DD, BB>), dim3((a.nrows + 2048 / DD - 1) / (2048 / DD)), dim3(256), 0,      \
+    hipLaunchKernelGGL((kv_read_mx_kernel<DD, BB>), dim3(blocks_for<DD>(a.nrows)), dim3(256), 0,                    \
                        stream, (const unsigned char*)k_codes, (const unsigned char*)k_scales,                        \
                        (const unsigned char*)v_codes, (const unsigned char*)v_scales, (bf16*)k_dst, (bf16*)v_dst,    \
                        ld_k, ld_v, a)

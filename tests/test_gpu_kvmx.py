@@ -373,3 +373,29 @@ def test_wrapper_refuses(ops):
     from mgen._lib import MgenError
     with pytest.raises(MgenError):
         step(wq=torch.ones(64, device=dev()))
+
+
+def test_more_rows_than_one_round_of_workgroups(ops):
+    """A call with more rows than 2^20 workgroups hold at once: its last rows."""
+    KVH, D, fmt = 8, 64, "mxfp4"
+    n = (1 << 22) + 3
+    w = KVH * D
+    g = torch.Generator().manual_seed(11)
+    tail = bf16_rows(g, 40, w)
+    rows = torch.zeros(n, w, dtype=torch.bfloat16, device=dev())
+    rows[-40:] = tail.to(dev())
+    kv = ops.MXKV.empty(1, KVH, n, D, fmt, dev())
+    for t in (kv.k, kv.k_scale, kv.v, kv.v_scale):
+        t.fill_(0xFF)
+    pos = torch.zeros(1, dtype=torch.int32, device=dev())
+    ops.kv_append_mx(rows, rows, w, w, kv, pos, 1, n)
+    code, e = K.quantise(tail.view(40, KVH, D).permute(1, 0, 2).double().numpy(), fmt)
+    for c, s in ((kv.k, kv.k_scale), (kv.v, kv.v_scale)):
+        assert np.array_equal(c[0, :, -40:].cpu().numpy(), K.pack(code, fmt))
+        assert np.array_equal(s[0, :, -40:].cpu().numpy(), e)
+        assert bool((s[0, :, :-40] == 1).all()) and bool((c[0, :, :-40] == 0).all())
+    back = torch.full((n, w), 7.0, dtype=torch.bfloat16, device=dev())
+    ops.kv_read_mx(kv, pos, back, rows, w, w, 1, n)
+    want = torch.from_numpy(K.values(K.pack(code, fmt), e, fmt)).bfloat16().permute(1, 0, 2).reshape(40, w)
+    assert torch.equal(back[-40:].cpu(), want) and torch.equal(rows[-40:], back[-40:])
+    assert bool((back[:-40] == 0).all())

@@ -1,6 +1,7 @@
 """Decode-only benchmark (GPU box): bench.py's two decode legs without the training step.
    python tools/bench_decode.py [repeats]      env: MGEN_DECODE_PARTS, MGEN_GEMM_SKINNY, LEGS=literal,long,short;
    MODEL=aria: the 650M Llama-style stand-in instead of the default decoder;
+   KV=mxfp8 | mxfp4: that KV cache instead of bf16 (the fractions printed then count the bf16 cache's bytes);
    GREEDY=1 replaces the sampler by the argmax (what the step costs without the top-p search and the draw)"""
 import os
 import sys
@@ -19,6 +20,11 @@ model = MidiLM(cfg, device=dev, seed=0)
 if os.environ.get("GREEDY") == "1":
     _generate = model.generate
     model.generate = lambda *a, **k: _generate(*a, **{**k, "do_sample": False})
+KV = os.environ.get("KV", "bf16")
+if KV != "bf16":
+    _plain, _reserve = model.generate, model.reserve_kv_cache
+    model.generate = lambda *a, **k: _plain(*a, **k, kv_cache=KV)
+    model.reserve_kv_cache = lambda streams, length: _reserve(streams, length, kv_cache=KV)
 for rep in range(int(sys.argv[1]) if len(sys.argv) > 1 else 1):
     legs = os.environ.get("LEGS", "literal,long").split(",")
     msg = []

@@ -8,25 +8,28 @@
 //
 // Bound: HBM. A key and its value are 2 (D/2 + D/32) bytes in 4 bits, read once for all query heads of their kv head.
 //
-// One workgroup per (key split, kv head with up to 8 query heads, stream); its waves walk units of keys.
+// One workgroup per (key split, kv head with up to 8 query heads, stream); its waves walk units of keys. A load instruction
+// is one contiguous kilobyte of codes (MXTiles).
 //
-// One query head per kv head (MXOne), all on the vector unit: a load instruction is one contiguous kilobyte, 16 bytes of
-// codes per lane (32 or 16 elements of one key, in one block), LR = 2, 4 or 8 lanes per row. Scores: codes to bf16 pairs,
-// two products and their sum per instruction, the LR lanes of a row add up. V: codes to fp32, weighted into the lane's own
-// sums (its elements, over its own keys). Keys meet after the loop.
+// One query head per kv head (MXOne), all on the vector unit. Scores: codes to bf16 pairs, two products and their sum per
+// instruction, the 2, 4 or 8 lanes of a row add up. V: codes to fp32, weighted into the lane's own sums (its elements, over
+// its own keys). Keys meet after the loop.
+//   256 streams x 8 heads x 128: 2048 keys in 8 bits 166 us (6.7 TB/s), 4096 in 4 bits 171 us (6.7), 2048 in 4 bits 91 (6.2).
 //
-// Several query heads (MXHeads), on the matrix cores: a wave walks two tiles of 16 keys; lane (r, g), r = lane & 15, g =
-// lane >> 4, takes the g-th quarter of key r's row, and its codes become bf16 operand fragments of 8 elements (exactly).
+// Several query heads (MXHeads), on the matrix cores: a unit of 32 keys goes from the loads' layout to the operands' through
+// LDS (as codes); lane (r, g), r = lane & 15, g = lane >> 4, then holds the g-th quarter of rows r and 16 + r, and its codes
+// become bf16 operand fragments of 8 elements (exactly).
 //  * Scores: the reduction runs over the elements in the order the lanes hold them, a permutation that q shares. The heads
 //    are the columns (columns i and 8 + i hold the same head): lane (r, g) ends up with column r, keys 4g .. 4g+3, which is
 //    the operand layout of the second product, so the weights never cross lanes.
 //  * The second product reduces over keys, so a lane needs V by element, not by key: the matrix cores turn the tile around
 //    (V fragment times a 0/1 selection of 16 of its 32 elements - one product per output, exact), a matrix instruction per
-//    16 x 16 elements of a pipe that is mostly idle here, instead of a round trip through LDS.
+//    16 x 16 elements of a pipe that is mostly idle here. (Through a bf16 image in LDS instead, read transposed: the same.)
 //  * Weights enter as two bf16 numbers, their rounded value in columns 0..7 and what that leaves in columns 8..15 (16 bits
 //    of weight at the price of 8); the two rows are added at the end.
 //  * A value block written with an infinity or a NaN enters as zeros and its elements of the result are set to NaN at the
 //    end (0 * NaN in the turning product would reach the other elements).
+//   256 streams x 8 kv heads of 4 x 128, 2048 keys in 4 bits 106 us (5.4 TB/s; a vector instruction mix of some 250 a unit).
 //
 // Both: the running maximum of a head is shared by the wave and moves only when a score exceeds it by more than 2^8 in the
 // weight (sums stay far inside fp32); then the sums are scaled. Sums, maxima and outputs are fp32. Rows outside the split
@@ -79,48 +82,105 @@ __device__ __forceinline__ rsrc_t mx_rsrc(const unsigned char* p, unsigned bytes
 struct MXRsrc {                          // the split's keys: codes and scales of K and V
     rsrc_t k, ks, v, vs;
 };
-__device__ __forceinline__ u32x4 mx_load16(rsrc_t r, int off, bool stream) {
-    return stream ? __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 2) : __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-}
 __device__ __forceinline__ f32x4 mx_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+// scale byte of block blk of a bf16 row
+template <int BITS>
+__device__ __forceinline__ unsigned mx_block_exponent(const bf16* row, int blk) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, mx_top8(*reinterpret_cast<const bf16x8*>(row + 32 * blk + 8 * i)));
+    return mx_exponent<BITS>(top);
+}
 
-// What a lane holds of a unit of T tiles: W dwords of codes of K and of V and their scale bytes
-template <int W, int T>
-struct MXUnit {
-    unsigned k[T][W], v[T][W], ke[T], ve[T];
+// How a wave reads codes: T tiles of KPT consecutive keys, each one contiguous kilobyte: 16 bytes per lane, ED elements of
+// one key inside one block, LR lanes a row. (Loads in the matrix cores' own layout - 16 neighbouring lanes in 16 rows - take
+// the address unit a clock per cache line for 16 bytes of it, 16 bytes a clock and CU: 4.9 TB/s at 256 x 2048 keys.)
+template <int D, int BITS, int T>
+struct MXTiles {
+    static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
+    static constexpr int LR = RB / 16, KPT = 64 / LR;
+    static constexpr int ED = 128 / BITS;             // elements of a lane
+    static constexpr int WF = BITS / 4;               // dwords of 8 elements
+
+    __device__ __forceinline__ static int key(int lane) { return lane / LR; }        // of a tile
+    __device__ __forceinline__ static int elem(int lane) { return lane % LR * ED; }
+    __device__ __forceinline__ static int block(int lane) { return elem(lane) / 32; }
+
+    template <int AUX>
+    __device__ __forceinline__ static void load(rsrc_t codes, int base, int lane, unsigned (&c)[T][4]) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(codes, (base + t * KPT) * RB + lane * 16, 0, AUX);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[t][i] = x[i];
+        }
+    }
+    // the codes of key t_new from its bf16 row, in the lanes that hold it; with `write` to the cache too (the row's codes
+    // and scale bytes). Returns the scale byte of the lane's block.
+    __device__ __forceinline__ static unsigned patch(unsigned (&c)[T][4], int t_new, int lane, const bf16* row, bool write,
+                                                     unsigned char* codes, unsigned char* scales) {
+        const unsigned e = mx_block_exponent<BITS>(row, block(lane));
+        unsigned x[4];
+#pragma unroll
+        for (int j = 0; j < ED / 8; ++j)
+            mx_encode8<BITS>(*reinterpret_cast<const bf16x8*>(row + elem(lane) + 8 * j), e, x + j * WF);
+        if (write) {
+            *reinterpret_cast<u32x4*>(codes + lane % LR * 16) = u32x4{x[0], x[1], x[2], x[3]};
+            scales[block(lane)] = (unsigned char)e;                 // (lanes of a block write the same byte)
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[t][i] = t == t_new / KPT ? x[i] : c[t][i];
+        return e;
+    }
 };
 
-// A core walks units of T tiles of KPT keys with the softmax state of its wave; its lane's part of a row consists of NP
-// pieces, each inside one block.
+// A core walks units of KPU keys with the softmax state of its wave.
 
 // One query head
 template <int D, int BITS>
 struct MXOne {
-    static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
-    static constexpr int LR = RB / 16;                // lanes of a row
-    static constexpr int KPT = 64 / LR, T = 4, W = 4, NP = 1, NW = 4;
-    // waves a SIMD has to hold; the step's instances in 4 bits would spill at the 128 registers that 4 waves leave
-    static constexpr int waves(int prep) { return BITS == 4 && prep ? 3 : 4; }
-    static constexpr int ED = 128 / BITS;             // elements of a lane
-    static constexpr int WF = BITS / 4;               // dwords of 8 elements
-
-    typedef MXUnit<W, T> Unit;
+    static constexpr int T = 4;
+    typedef MXTiles<D, BITS, T> R;
+    static constexpr int KPT = R::KPT, KPU = T * KPT, LR = R::LR, ED = R::ED, WF = R::WF, NB = R::NB;
+    static constexpr int IMG = 0;                     // bytes of LDS a wave works in
+    static constexpr int WAVES = 4;                   // a SIMD has to hold
+    struct Unit {                                     // codes and scale bytes of K and of V
+        unsigned k[T][4], v[T][4], ke[T], ve[T];
+    };
     bf16x2 q[ED / 2];
     float m, l, acc[ED], sl2;
     int lane;
 
-    __device__ __forceinline__ void place(int lane_) { lane = lane_; }
-    __device__ __forceinline__ int key() const { return lane / LR; }                       // of a tile
-    __device__ __forceinline__ int elem(int j) const { return lane % LR * ED + 8 * j; }    // of the lane's j-th eight
-    __device__ __forceinline__ int block(int) const { return lane % LR * ED / 32; }
-
+    __device__ __forceinline__ void place(int lane_, char*) { lane = lane_; }
+    __device__ __forceinline__ int key() const { return R::key(lane); }
+    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) const {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int at = (base + t * KPT + key()) * NB + R::block(lane);
+            u.ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at, 0, 0);
+            u.ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at, 0, 0);
+        }
+        // (read once: the non-temporal hint is worth 8 to 10 %)
+        R::template load<2>(s.k, base, lane, u.k);
+        R::template load<2>(s.v, base, lane, u.v);
+    }
+    // the step's own key t_new of the unit: K (codes c, scale bytes e) or V from its bf16 row
+    __device__ __forceinline__ void patch(unsigned (&c)[T][4], unsigned (&e)[T], int t_new, const bf16* row, bool write,
+                                          unsigned char* codes, unsigned char* scales) const {
+        if (key() != t_new % KPT) return;
+        const unsigned b = R::patch(c, t_new, lane, row, write, codes, scales);
+#pragma unroll
+        for (int t = 0; t < T; ++t) e[t] = t == t_new / KPT ? b : e[t];
+    }
     __device__ __forceinline__ void start(const bf16* src, int nh, float scale_log2e) {
         sl2 = scale_log2e;
 #pragma unroll
         for (int j = 0; j < ED / 8; ++j) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(src + elem(j));
+            const u32x4 x = *reinterpret_cast<const u32x4*>(src + R::elem(lane) + 8 * j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const unsigned w = x[i];
@@ -131,20 +191,6 @@ struct MXOne {
         l = 0.f;
 #pragma unroll
         for (int e = 0; e < ED; ++e) acc[e] = 0.f;
-    }
-    __device__ __forceinline__ void load(rsrc_t codes, rsrc_t scales, int base, unsigned (&c)[T][W], unsigned (&e)[T]) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const int at = base + t * KPT;
-            e[t] = __builtin_amdgcn_raw_buffer_load_b8(scales, at * NB + key() * NB + block(0), 0, 0);
-            const u32x4 x = mx_load16(codes, at * RB + lane * 16, true);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[t][i] = x[i];
-        }
-    }
-    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) {
-        load(s.k, s.ks, base, u.k, u.ke);
-        load(s.v, s.vs, base, u.v, u.ve);
     }
     // LAST: the unit with the split's last key, `left` keys from its first on
     template <bool LAST>
@@ -186,7 +232,7 @@ struct MXOne {
             l += w;
             const float sc = mx_scale(u.ve[t]);
 #pragma unroll
-            for (int x = 0; x < W; ++x) {
+            for (int x = 0; x < 4; ++x) {
                 constexpr int PW = 32 / BITS;
                 float f[PW];
                 mx_decode_f32<BITS>(u.v[t][x], sc, f);
@@ -198,7 +244,7 @@ struct MXOne {
     // The wave's maximum, denominator and sums to ml[2] and o[D]. Lanes that hold the same elements (64 / LR keys) add up,
     // halving the elements a lane is responsible for at every step: a swap of half waves or of neighbouring rows of 16
     // lanes brings two elements' halves together, then exchanges inside a row.
-    __device__ __forceinline__ void finish(float* ml, float* o, int nh, int hc) {
+    __device__ __forceinline__ void finish(float* ml, float* o, int nh) {
         l = wave64_sum(l);
         int from = lane % LR * ED;
 #pragma unroll
@@ -234,43 +280,89 @@ struct MXOne {
     }
 };
 
-// Up to MX_HEADS query heads. A lane's quarter of a row comes in NP pieces of at most 16 bytes: a load instruction takes
-// piece p of all 16 rows of a tile, 64 (32) contiguous bytes of every row.
+// Up to MX_HEADS query heads
 template <int D, int BITS>
 struct MXHeads {
     static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
-    static constexpr int KPT = 16, T = 2, W = RB / 16, NW = 8;
-    static constexpr int waves(int) { return 2; }
-    static constexpr int NP = RB == 128 ? 2 : 1;
-    static constexpr int PB = RB / 4 / NP;            // bytes of a piece
-    static constexpr int PD = D / 4 / NP;             // elements of a piece
+    static constexpr int KPU = 32, T = KPU / MXTiles<D, BITS, 1>::KPT;
+    typedef MXTiles<D, BITS, T> R;
+    static constexpr int W = RB / 16;                 // dwords of a quarter row
     static constexpr int NF = D / 32;                 // fragments of 8 elements
     static constexpr int WF = BITS / 4;               // dwords of a fragment
-
-    typedef MXUnit<W, T> Unit;            // (ke, ve: one byte, or with two pieces the row's four)
+    static constexpr int IMG = KPU * RB;              // bytes of LDS a wave works in: the codes of a unit
+    static constexpr int WAVES = RB == 128 ? 3 : 4;   // a SIMD has to hold (more registers than 4 leave where T is 4)
+    struct Unit {                                     // codes as they were loaded; scale bytes of a lane's quarter rows
+        unsigned k[T][4], v[T][4], ke[2], ve[2];
+    };
     bf16x8 qf[NF], pick[2];
     float m, l, sl2, low;                 // of column r; low: the column takes the weights' remainders
     f32x4 acc[NF][2];                     // rows = columns of the scores, column r of selection c
-    unsigned long long bad[NP];           // lanes that met a value block of scale 255, by piece
-    int r, g;
+    unsigned long long bad;               // lanes that met a value block of scale 255
+    char* img;
+    int lane, r, g;
 
-    __device__ __forceinline__ void place(int lane) {
+    __device__ __forceinline__ void place(int lane_, char* image) {
+        lane = lane_;
         r = lane & 15;
         g = lane >> 4;
+        img = image;
     }
-    __device__ __forceinline__ int key() const { return r; }
-    __device__ __forceinline__ static int elem_of(int j, int g) { return (j * 8 / PD) * 4 * PD + g * PD + j * 8 % PD; }
+    __device__ __forceinline__ static int elem_of(int j, int g) { return g * (D / 4) + 8 * j; }
     __device__ __forceinline__ int elem(int j) const { return elem_of(j, g); }
-    __device__ __forceinline__ int block(int p) const { return (p * 4 * PD + g * PD) / 32; }
-    __device__ __forceinline__ unsigned byte(unsigned e, int p) const { return NP == 1 ? e : (e >> (8 * block(p))) & 255u; }
+    __device__ __forceinline__ int block() const { return g * NB / 4; }
+
+    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int at = (base + 16 * t + r) * NB + block();
+            u.ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at, 0, 0);
+            u.ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at, 0, 0);
+        }
+        R::template load<2>(s.k, base, lane, u.k);
+        R::template load<2>(s.v, base, lane, u.v);
+    }
+    __device__ __forceinline__ void patch(unsigned (&c)[T][4], unsigned (&e)[2], int t_new, const bf16* row, bool write,
+                                          unsigned char* codes, unsigned char* scales) const {
+        if (R::key(lane) == t_new % R::KPT) R::patch(c, t_new, lane, row, write, codes, scales);
+        if (r == (t_new & 15)) {
+            const unsigned b = mx_block_exponent<BITS>(row, block());
+#pragma unroll
+            for (int t = 0; t < 2; ++t) e[t] = t == t_new >> 4 ? b : e[t];
+        }
+    }
+    // 16-byte chunk c of a row of the image, spread so that 16 rows' chunks lie on different banks
+    __device__ __forceinline__ static int at(int row, int c) {
+        return row * RB + 16 * (c ^ (RB == 128 ? row >> 1 & 7 : RB == 64 ? row >> 2 & 3 : row >> 3 & 1));
+    }
+    // from the loads' layout to the lane's quarters of key r of both tiles, through the wave's image
+    __device__ __forceinline__ void spread(const unsigned (&c)[T][4], unsigned (&out)[2][W]) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+            lds_write_b128(img, at(t * R::KPT + R::key(lane), lane % R::LR), u32x4{c[t][0], c[t][1], c[t][2], c[t][3]});
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int row = 16 * t + r;
+            if (W == 2) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(img + at(row, g >> 1) + 8 * (g & 1));
+                out[t][0] = x[0];
+                out[t][1] = x[1];
+            } else {
+#pragma unroll
+                for (int h = 0; h < W / 4; ++h) {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(img + at(row, g * (W / 4) + h));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[t][4 * h + i] = x[i];
+                }
+            }
+        }
+    }
 
     __device__ __forceinline__ void start(const bf16* q, int nh, float scale_log2e) {
         sl2 = scale_log2e;
         low = r >> 3 ? 1.f : 0.f;
         m = MX_LOW;
         l = 0.f;
-#pragma unroll
-        for (int p = 0; p < NP; ++p) bad[p] = 0;
+        bad = 0;
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
             qf[j] = bf16x8{};
@@ -286,42 +378,16 @@ struct MXHeads {
 #pragma unroll
             for (int c = 0; c < 2; ++c) acc[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ static void load_row(rsrc_t s, int off, unsigned* out) {
-        if (W == 2) {
-            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(s, off, 0, 0);
-            out[0] = x[0];
-            out[1] = x[1];
-        } else {
-#pragma unroll
-            for (int h = 0; h < W / 4; ++h) {
-                const u32x4 x = mx_load16(s, off + 4 * PB * h, false);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) out[4 * h + i] = x[i];
-            }
-        }
-    }
-    __device__ __forceinline__ void load(rsrc_t codes, rsrc_t scales, int base, unsigned (&c)[T][W], unsigned (&e)[T]) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const int at = base + 16 * t + r;
-            if (NP == 1) e[t] = __builtin_amdgcn_raw_buffer_load_b8(scales, at * NB + block(0), 0, 0);
-            else e[t] = __builtin_amdgcn_raw_buffer_load_b32(scales, at * NB, 0, 0);
-            load_row(codes, at * RB + g * PB, c[t]);
-        }
-    }
-    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) {
-        load(s.k, s.ks, base, u.k, u.ke);
-        load(s.v, s.vs, base, u.v, u.ve);
-    }
     template <bool LAST>
     __device__ __forceinline__ void unit(const Unit& u, int left) {
         float s[8];
+        unsigned c[2][W];
+        spread(u.k, c);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < NF; ++j)
-                a = mx_mfma(mx_decode8<BITS>(u.k[t] + j * WF, mx_scale(byte(u.ke[t], j * 8 / PD))), qf[j], a);
+            for (int j = 0; j < NF; ++j) a = mx_mfma(mx_decode8<BITS>(c[t] + j * WF, mx_scale(u.ke[t])), qf[j], a);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[4 * t + i] = a[i] * sl2;
@@ -355,34 +421,31 @@ struct MXHeads {
             l += w;
             p[i] = (bf16)fmaf(-low, round_bf(w), w);
         }
-        float vs[2][NP];
+        spread(u.v, c);
+        float vs[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int x = 0; x < NP; ++x) {
-                const unsigned e = byte(u.ve[t], x);
-                bad[x] |= __ballot(e == 255u);
-                vs[t][x] = e == 255u ? 0.f : mx_scale(e);
-            }
+        for (int t = 0; t < 2; ++t) {
+            bad |= __ballot(u.ve[t] == 255u);
+            vs[t] = u.ve[t] == 255u ? 0.f : mx_scale(u.ve[t]);
+        }
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
-            const bf16x8 v0 = mx_decode8<BITS>(u.v[0] + j * WF, vs[0][j * 8 / PD]);
-            const bf16x8 v1 = mx_decode8<BITS>(u.v[1] + j * WF, vs[1][j * 8 / PD]);
+            const bf16x8 v0 = mx_decode8<BITS>(c[0] + j * WF, vs[0]), v1 = mx_decode8<BITS>(c[1] + j * WF, vs[1]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int b = 0; b < 2; ++b) {
                 const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                const f32x4 t0 = mx_mfma(v0, pick[c], zero), t1 = mx_mfma(v1, pick[c], zero);   // keys 4g + i, column r
+                const f32x4 t0 = mx_mfma(v0, pick[b], zero), t1 = mx_mfma(v1, pick[b], zero);   // keys 4g + i, column r
                 bf16x8 x;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     x[i] = (bf16)t0[i];
                     x[4 + i] = (bf16)t1[i];
                 }
-                acc[j][c] = mx_mfma(p, x, acc[j][c]);
+                acc[j][b] = mx_mfma(p, x, acc[j][b]);
             }
         }
     }
-    __device__ __forceinline__ void finish(float* ml, float* o, int nh, int hc) {
+    __device__ __forceinline__ void finish(float* ml, float* o, int nh) {
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (g == 0 && r < nh) {
@@ -394,7 +457,7 @@ struct MXHeads {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int from = 2 * c + (r >> 3);                  // lanes g the column's element came from
-                const float nan = (bad[j * 8 / PD] >> (16 * from)) & 0xFFFFu ? __uint_as_float(0x7FC00000u) : 0.f;
+                const float nan = (bad >> (16 * from)) & 0xFFFFu ? __uint_as_float(0x7FC00000u) : 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {                       // rows 8 + i hold the remainders
                     const float x = acc[j][c][i] + __shfl_xor(acc[j][c][i], 32, 64) + nan;
@@ -408,24 +471,25 @@ struct MXHeads {
 // the new key and the new value come from the raw projection rows; the new row is quantised, takes the place of key
 // kv_len[b] - 1 in the lanes that own it, and is written to the cache by the first head group.
 template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
-__global__ __launch_bounds__(64 * NW, (Core<D, BITS>::waves(PREP))) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
+__global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
                                                                  const int* __restrict__ kv_len, int H, int KVH,
                                                                  int nsplit, float scale, float* __restrict__ part_ml,
                                                                  float* __restrict__ part_o, bf16* __restrict__ out,
                                                                  long ld_o, MXPrep pp) {
     typedef Core<D, BITS> C;
-    constexpr int RB = C::RB, NB = C::NB, KPT = C::KPT, KPU = C::T * KPT;
+    constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB, KPU = C::KPU;
     extern __shared__ __attribute__((aligned(16))) float smem[];
 
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS;
     const int split = blockIdx.x, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
     const int h0 = kvh * group + chunk * MX_HEADS, nh = min(MX_HEADS, group - chunk * MX_HEADS), hc = min(MX_HEADS, group);
-    bf16* sm_q = reinterpret_cast<bf16*>(smem);      // [hc + 2][D]: q heads, new key, new value (PREP); gives way to
-    float* sm_o = smem;                              // [NW][hc][D] and
+    // LDS: q heads, new key and new value (PREP) and what the cores work in, which then give way to the waves' sums
+    bf16* sm_q = reinterpret_cast<bf16*>(smem + NW * C::IMG / 4);    // [hc + 2][D]
+    float* sm_o = smem;                              // [NW][hc][D]
     float* sm_ml = smem + NW * hc * D;               // [NW][hc][2]
     const int tid = threadIdx.x, wave = tid >> 6;
     C core;
-    core.place(tid & 63);
+    core.place(tid & 63, reinterpret_cast<char*>(smem) + wave * C::IMG);
 
     const int len = mx_length<PREP>(kv_len, kv.max_len, pp, b), pos = len - 1;       // (pos: of the new token, PREP)
     if (len <= 0) {                       // a stream without keys: zeros
@@ -476,45 +540,18 @@ __global__ __launch_bounds__(64 * NW, (Core<D, BITS>::waves(PREP))) void attn_de
     if (base < n) {
         core.load(src, base, u);
         const int t_new = n - 1 - base;   // the stream's last key, in its last split
-        if (PREP && k_beg + n == len && core.key() == t_new % KPT) {
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                const bf16* row = sm_q + (hc + which) * D;
-                unsigned char* codes = const_cast<unsigned char*>(which ? kv.v : kv.k) + (slice + pos) * RB;
-                unsigned char* scales = const_cast<unsigned char*>(which ? kv.vs : kv.ks) + (slice + pos) * NB;
-                unsigned c[C::W], all = 0;
-#pragma unroll
-                for (int j = 0; j < C::W / C::WF; ++j) {
-                    constexpr int PER = C::W / C::WF / C::NP;       // eights of a piece
-                    const int blk = core.block(j / PER);
-                    unsigned top = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        top = max(top, mx_top8(*reinterpret_cast<const bf16x8*>(row + 32 * blk + 8 * i)));
-                    const unsigned e = mx_exponent<BITS>(top);
-                    mx_encode8<BITS>(*reinterpret_cast<const bf16x8*>(row + core.elem(j)), e, c + j * C::WF);
-                    if (j % PER == 0) all |= C::NP == 1 ? e : e << (8 * blk);
-                    if (chunk == 0) {
-#pragma unroll
-                        for (int x = 0; x < C::WF; ++x)
-                            *reinterpret_cast<unsigned*>(codes + core.elem(j) * BITS / 8 + 4 * x) = c[j * C::WF + x];
-                        scales[blk] = (unsigned char)e;             // (lanes that share a block write the same byte)
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < C::T; ++t)
-                    if (t == t_new / KPT) {
-#pragma unroll
-                        for (int x = 0; x < C::W; ++x) (which ? u.v : u.k)[t][x] = c[x];
-                        (which ? u.ve : u.ke)[t] = all;
-                    }
-            }
+        if (PREP && k_beg + n == len) {
+            const long at = slice + pos;
+            core.patch(u.k, u.ke, t_new, sm_q + hc * D, chunk == 0, const_cast<unsigned char*>(kv.k) + at * RB,
+                       const_cast<unsigned char*>(kv.ks) + at * NB);
+            core.patch(u.v, u.ve, t_new, sm_q + (hc + 1) * D, chunk == 0, const_cast<unsigned char*>(kv.v) + at * RB,
+                       const_cast<unsigned char*>(kv.vs) + at * NB);
         }
         core.template unit<true>(u, n - base);
     }
 
-    if (PREP) __syncthreads();            // sm_q lies where the sums go
-    core.finish(sm_ml + wave * hc * 2, sm_o + wave * hc * D, nh, hc);
+    if (PREP || C::IMG) __syncthreads();  // the sums overwrite both
+    core.finish(sm_ml + wave * hc * 2, sm_o + wave * hc * D, nh);
     __syncthreads();
 #pragma unroll 1
     for (int x = tid; x < nh * D; x += 64 * NW) {
@@ -595,14 +632,14 @@ __global__ __launch_bounds__(256) void attn_decode_mx_merge_kernel(const float* 
     }
 }
 
-template <int D, int BITS, int PREP, template <int, int> class Core>
+template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
 void launch(const void* q, long ld_q, MXView kv, const int* kv_len, void* out, long ld_o, float* ws, int B, int H,
             int KVH, int nsplit, float scale, MXPrep pp, hipStream_t stream) {
-    constexpr int NW = Core<D, BITS>::NW;
     float* part_ml = ws;
     float* part_o = ws ? ws + (long)B * H * nsplit * 2 : nullptr;
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS, hc = group < MX_HEADS ? group : MX_HEADS;
-    const int lds = NW * hc * (D + 2) * 4;           // (more than the PREP rows: (hc + 2) * D * 2 bytes)
+    const int loop = NW * Core<D, BITS>::IMG + (PREP ? (hc + 2) * D * 2 : 0), sums = NW * hc * (D + 2) * 4;
+    const int lds = loop > sums ? loop : sums;
     hipLaunchKernelGGL((attn_decode_mx_kernel<D, BITS, PREP, Core, NW>), dim3(nsplit, KVH * chunks, B), dim3(64 * NW), lds,
                        stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, scale, part_ml, part_o, (bf16*)out, ld_o,
                        pp);
@@ -629,10 +666,14 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
     MGEN_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (D / 32 - 1)) == 0, "%s: scales must be aligned to a row (D / 32)", what);
     const MXView kv{(const unsigned char*)kc, (const unsigned char*)ks, (const unsigned char*)vc,
                     (const unsigned char*)vs, max_len};
+    // Several heads: 8 waves where a CU gets one workgroup or none (1 stream of 100003 keys, 4 kv heads of 4, 64 splits: 25 us
+    // against 29 in workgroups of 4; 32 x 8 kv heads of 8, 4096 keys: 48 and 54), 4 beyond (96 x 24, 3 keys: 27 and 14).
 #define LAUNCH(DD, BB)                                                                                                 \
     do {                                                                                                               \
-        if (H == KVH) launch<DD, BB, PREP, MXOne>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
-        else launch<DD, BB, PREP, MXHeads>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream);  \
+        if (H == KVH) launch<DD, BB, PREP, MXOne, 4>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
+        else if ((long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS) * nsplit <= 256)                                \
+            launch<DD, BB, PREP, MXHeads, 8>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
+        else launch<DD, BB, PREP, MXHeads, 4>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream);  \
     } while (0)
     if (D == 128) { if (bits == 4) LAUNCH(128, 4); else LAUNCH(128, 8); }
     else { if (bits == 4) LAUNCH(64, 4); else LAUNCH(64, 8); }
@@ -643,23 +684,24 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 }  // namespace
 
 // Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
-// Few workgroups: as many splits as bring them to 512, each with keys for two rounds of its waves (several heads: one) or
+// Few workgroups: as many splits as bring them to 512 (several heads: 1024), each with keys for two rounds of its waves or
 // more, where the second launch is worth its 3 us: from 8 rounds on (1 stream x 8 heads x 128 in 8 bits: 4096 keys, 32
-// rounds, 24.5 us in one split and 7.4 in 16; 512 keys, 4 rounds, 5.4 and 7.2).
+// rounds, 24.5 us in one split and 7.4 in 16; 512 keys, 4 rounds, 5.4 and 7.2. 16 streams of up to 8192 keys, 8 kv heads of
+// 4: 27 us in 4 splits, 23 in 8).
 // Many: one, unless that leaves the last round of the chip's 1024 places less than 7/8 full (64 streams x 24 heads x 2047
 // keys: 1536 workgroups, 79 us in one split and 70 in two; 256 x 8: 166 and 172).
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
     if (B <= 0 || KVH <= 0 || H < KVH || longest <= 0) return 1;
+    const bool one = H == KVH;
     const long groups = (long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS);
-    // keys of one round of a workgroup's waves, taken at 8 bits
-    const int round = H == KVH ? (D == 128 ? 128 : 256) : 256;
+    const int round = one && D == 64 ? 256 : 128;     // keys of a round of a workgroup's waves, taken at 8 bits
     const int rounds = (longest + round - 1) / round;
     if (rounds < 8) return 1;
     if (groups < 256) {
-        const long n = 512 / groups, most = H == KVH ? rounds / 2 : rounds;
+        const long n = (one ? 512 : 1024) / groups, most = rounds / 2;
         return (int)(n < most ? (n < MX_MAX_SPLITS ? n : MX_MAX_SPLITS) : most < MX_MAX_SPLITS ? most : MX_MAX_SPLITS);
     }
-    if (groups > 1024)
+    if (one && groups > 1024)
         for (int n = 1; n <= 4; ++n) {
             const long wg = groups * n, places = (wg + 1023) / 1024 * 1024;
             if (8 * wg >= 7 * places) return n;

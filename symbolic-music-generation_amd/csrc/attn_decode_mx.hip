@@ -9,7 +9,8 @@
 // Bound: HBM. A key and its value are 2 (D/2 + D/32) bytes in 4 bits, read once for all query heads of their kv head.
 //
 // One workgroup per (key split, kv head with up to 8 query heads, stream); its waves walk units of keys. A load instruction
-// is one contiguous kilobyte of codes (MXTiles).
+// is one contiguous kilobyte of codes (MXTiles). Streams of different lengths: 256 x 8 heads x 128, 1 to 4096 keys in 4 bits
+// 97 us (6.0 TB/s; the same number of keys in equal streams 93).
 //
 // One query head per kv head (MXOne), all on the vector unit. Scores: codes to bf16 pairs, two products and their sum per
 // instruction, the 2, 4 or 8 lanes of a row add up. V: codes to fp32, weighted into the lane's own sums (its elements, over
@@ -45,6 +46,9 @@ constexpr float MX_LOW = -3.0e38f;      // below every finite score that matters
 constexpr float MX_SLACK = 8.0f;
 constexpr int MX_HEADS = 8;            // query heads of a workgroup
 constexpr int MX_MAX_SPLITS = 64;      // (a lane of one wave each in the joining kernel)
+constexpr int MX_PLACES = 1024;        // workgroups on the chip at a time
+constexpr int MX_ORDERED = 512;        // streams that a workgroup puts in order
+constexpr int MX_ORDER_KEYS = 1024;    // capacity from which on that pays
 constexpr int MX_MIN_SPLIT = 256;      // keys below which a split is not worth a workgroup
 
 struct MXView {
@@ -68,6 +72,46 @@ __device__ __forceinline__ int mx_length(const int* kv_len, int max_len, const M
     if (!PREP) return min(len, max_len);
     const int pos = pp.pos[b];
     return pos < 0 || pos >= max_len || pos >= pp.npos || len != pos + 1 ? 0 : len;
+}
+// The n streams from `first` on in the order of their keys, the longest first (to 1/256 of the longest one's; equal ones as
+// they are numbered): the stream of rank `rank` among them, found bit by bit as the largest length that more than `rank`
+// streams reach. Every lane of a wave calls it and gets the same answer.
+__device__ __forceinline__ int mx_by_length(const int* kv_len, int max_len, int first, int n, int rank, int lane) {
+    constexpr int NL = MX_ORDERED / 64;
+    int key[NL];
+    float longest = 1.f;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        key[i] = -1;
+        if (i * 64 + lane < n) key[i] = max(min(kv_len[first + i * 64 + lane], max_len), 0);
+        longest = fmaxf(longest, (float)key[i]);
+    }
+    const float unit = 255.9f / wave64_max(longest);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) key[i] = key[i] < 0 ? -1 : (int)((float)key[i] * unit);
+    int at = 0, above = 0;                // streams of key at or more: above rank; of more than that: `above`
+#pragma unroll 1
+    for (int bit = 128; bit; bit >>= 1) {
+        int k = 0;
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (i * 64 < n) k += __popcll(__ballot(key[i] >= at + bit));
+        if (k > rank) at += bit;
+        else above = k;
+    }
+    rank -= above;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const bool in = key[i] == at;
+        const unsigned long long m = __ballot(in);
+        const int k = __popcll(m);
+        if (rank < k) {
+            const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0));
+            return first + i * 64 + __ffsll(__ballot(in && before == rank)) - 1;
+        }
+        rank -= k;
+    }
+    return first;                         // (not reached: rank < n)
 }
 // keys of a split of a stream of len: short streams use fewer of the splits
 __device__ __forceinline__ int mx_split(int len, int nsplit) {
@@ -473,7 +517,8 @@ struct MXHeads {
 template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
 __global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_mx_kernel(const bf16* __restrict__ q, long ld_q, MXView kv,
                                                                  const int* __restrict__ kv_len, int H, int KVH,
-                                                                 int nsplit, float scale, float* __restrict__ part_ml,
+                                                                 int nsplit, int first, float scale,
+                                                                 float* __restrict__ part_ml,
                                                                  float* __restrict__ part_o, bf16* __restrict__ out,
                                                                  long ld_o, MXPrep pp) {
     typedef Core<D, BITS> C;
@@ -481,7 +526,10 @@ __global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_m
     extern __shared__ __attribute__((aligned(16))) float smem[];
 
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS;
-    const int split = blockIdx.x, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
+    const int split = blockIdx.x, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
+    int b = blockIdx.z;
+    if (b >= first) b = __builtin_amdgcn_readfirstlane(mx_by_length(kv_len, kv.max_len, first, gridDim.z - first, b - first,
+                                                                    threadIdx.x & 63));
     const int h0 = kvh * group + chunk * MX_HEADS, nh = min(MX_HEADS, group - chunk * MX_HEADS), hc = min(MX_HEADS, group);
     // LDS: q heads, new key and new value (PREP) and what the cores work in, which then give way to the waves' sums
     bf16* sm_q = reinterpret_cast<bf16*>(smem + NW * C::IMG / 4);    // [hc + 2][D]
@@ -640,8 +688,14 @@ void launch(const void* q, long ld_q, MXView kv, const int* kv_len, void* out, l
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS, hc = group < MX_HEADS ? group : MX_HEADS;
     const int loop = NW * Core<D, BITS>::IMG + (PREP ? (hc + 2) * D * 2 : 0), sums = NW * hc * (D + 2) * 4;
     const int lds = loop > sums ? loop : sums;
+    // More workgroups than the chip holds: behind the streams that start at once (their order does not matter, and it would
+    // show as latency) the longest go first, or a long one that starts last runs on alone. 256 x 8 heads x 128, lengths up
+    // to 4096: 4 bits 106 us as numbered, 97 ordered; with 4 heads per kv head 124 and 110; lengths up to 2048 in 8 bits 118
+    // and 108; equal lengths 168 and 169. Short caches end before it pays (96 x 24 heads, 3 keys: 14.0 and 17.5).
+    const long groups = (long)KVH * chunks * nsplit, at_once = MX_PLACES / groups;
+    const int first = kv.max_len >= MX_ORDER_KEYS && B > at_once && B - at_once <= MX_ORDERED ? (int)at_once : B;
     hipLaunchKernelGGL((attn_decode_mx_kernel<D, BITS, PREP, Core, NW>), dim3(nsplit, KVH * chunks, B), dim3(64 * NW), lds,
-                       stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, scale, part_ml, part_o, (bf16*)out, ld_o,
+                       stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, first, scale, part_ml, part_o, (bf16*)out, ld_o,
                        pp);
     if (nsplit > 1)
         hipLaunchKernelGGL((attn_decode_mx_merge_kernel<D, PREP>), dim3(H, B), dim3(256), 0, stream, part_ml, part_o, kv_len,

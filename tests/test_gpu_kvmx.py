@@ -433,3 +433,33 @@ def test_workspace_on_the_cache_device(ops):
     n = torch.ones(1, dtype=torch.int32, device=dev())
     with pytest.raises(ValueError, match="workspace"):
         ops.attn_decode_mx(rows, 128, kv, n, rows.clone(), 128, torch.empty(4096), 1, 2, 2, 0.1)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("B,H,KVH,nsplit,step", [(140, 8, 8, 1, 70), (150, 16, 8, 1, 75), (530, 8, 8, 1, 106), (645, 8, 8, 1, 100),
+                                                 (90, 8, 8, 2, 40), (1100, 2, 1, 1, 550)])
+def test_order_of_the_streams_does_not_show(ops, fmt, B, H, KVH, nsplit, step):
+    """Streams of different lengths in a call with more workgroups than the chip holds, which takes long ones first: the bits
+    of calls that take them as they are numbered; every row is written."""
+    D, L = 64, 1030
+    g = torch.Generator().manual_seed(B)
+    kv = ops.MXKV.empty(B, KVH, L, D, fmt, dev())
+    rows = bf16_rows(g, L, KVH * D, spread=1).to(dev())
+    ops.kv_append_mx(rows.repeat(8, 1), rows.flip(0).repeat(8, 1), KVH * D, KVH * D, kv, torch.zeros(8, dtype=torch.int32,
+                     device=dev()), 8, L)
+    for t in (kv.k, kv.k_scale, kv.v, kv.v_scale):
+        t[8:] = t[:1]
+    lens = torch.randint(0, L + 1, (B,), generator=g, dtype=torch.int32)
+    lens[::5] = 700                                      # equal ones
+    lens[3::7] = torch.tensor([0, 1, L, L + 9, -2], dtype=torch.int32).repeat(B)[:lens[3::7].numel()]
+    lens = lens.to(dev())
+    q = bf16_rows(g, B, H * D, spread=1).to(dev())
+    ws = torch.empty(ops.attn_decode_workspace(B, H, D, nsplit), dtype=torch.float32, device=dev())
+    whole, parts = (torch.full((B, H * D), 7.0, dtype=torch.bfloat16, device=dev()) for _ in range(2))
+    ops.attn_decode_mx(q, H * D, kv, lens, whole, H * D, ws, B, H, nsplit, D ** -0.5)
+    for b in range(0, B, step):
+        e = min(b + step, B)
+        ops.attn_decode_mx(q[b:e], H * D, kv.streams(b, e), lens[b:e], parts[b:e], H * D, ws, e - b, H, nsplit, D ** -0.5)
+    assert torch.equal(whole, parts)
+    assert not bool((whole == 7.0).all(-1).any())
+    assert bool((whole[lens <= 0] == 0).all())

@@ -740,27 +740,19 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 // Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
 // Few workgroups: as many splits as bring them to 512 (several heads: 1024), each with keys for two rounds of its waves or
 // more, where the second launch is worth its 3 us: from 8 rounds on (1 stream x 8 heads x 128 in 8 bits: 4096 keys, 32
-// rounds, 24.5 us in one split and 7.4 in 16; 512 keys, 4 rounds, 5.4 and 7.2. 16 streams of up to 8192 keys, 8 kv heads of
-// 4: 27 us in 4 splits, 23 in 8).
-// Many: one, unless that leaves the last round of the chip's 1024 places less than 7/8 full (64 streams x 24 heads x 2047
-// keys: 1536 workgroups, 79 us in one split and 70 in two; 256 x 8: 166 and 172).
+// rounds, 33 us in one split and 8.3 in 16; 512 keys, 4 rounds, 5.7 and 7.6. 16 streams of up to 8192 keys, 8 kv heads of
+// 4: 27 us in 4 splits, 24 in 8).
+// From 256 workgroups on: one (two, at 1500 keys: 1536 workgroups of heads of 64 in 4 bits 28 and 38 us, in 8 bits 50 and 52,
+// of 128 96 and 99; at 6000 keys 347 and 355).
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
     if (B <= 0 || KVH <= 0 || H < KVH || longest <= 0) return 1;
     const bool one = H == KVH;
     const long groups = (long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS);
     const int round = one && D == 64 ? 256 : 128;     // keys of a round of a workgroup's waves, taken at 8 bits
     const int rounds = (longest + round - 1) / round;
-    if (rounds < 8) return 1;
-    if (groups < 256) {
-        const long n = (one ? 512 : 1024) / groups, most = rounds / 2;
-        return (int)(n < most ? (n < MX_MAX_SPLITS ? n : MX_MAX_SPLITS) : most < MX_MAX_SPLITS ? most : MX_MAX_SPLITS);
-    }
-    if (one && groups > 1024)
-        for (int n = 1; n <= 4; ++n) {
-            const long wg = groups * n, places = (wg + 1023) / 1024 * 1024;
-            if (8 * wg >= 7 * places) return n;
-        }
-    return 1;
+    if (rounds < 8 || groups >= 256) return 1;
+    const long n = (one ? 512 : 1024) / groups, most = rounds / 2;
+    return (int)(n < most ? (n < MX_MAX_SPLITS ? n : MX_MAX_SPLITS) : most < MX_MAX_SPLITS ? most : MX_MAX_SPLITS);
 }
 
 // q [B][ld_q] (heads at h*D), out [B][ld_o] bf16; kv_len[b] = cached keys of stream b (0: the output row is zeros; values

@@ -23,15 +23,16 @@ def use_stream(handle):
     _stream_override = handle
 
 
-# the handle of the current stream without the Stream object around it (0.3 against 2.8 us a call, on every launch)
+# the handle of the current stream without the Stream object around it (0.2 against 2.8 us a call, on every launch)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream():
     if _stream_override is not None:
         return _stream_override
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -619,7 +620,7 @@ class MXKV:
     """One layer's keys and values in blocks of 32 elements with a shared power-of-two scale (include/mgen.h, "KV cache in
     4 or 8 bits"): codes k, v uint8 [B, KVH, max_len, D or D/2], scales k_scale, v_scale uint8 [B, KVH, max_len, D/32]."""
 
-    __slots__ = ("k", "k_scale", "v", "v_scale", "B", "KVH", "max_len", "D", "bits", "fmt", "device", "ptrs")
+    __slots__ = ("k", "k_scale", "v", "v_scale", "B", "KVH", "max_len", "D", "bits", "fmt", "device", "index", "ptrs")
 
     def __init__(self, k, k_scale, v, v_scale):
         for t in (k, k_scale, v, v_scale):
@@ -641,7 +642,7 @@ class MXKV:
         _need_gpu(k)
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
         self.fmt = "mxfp4" if self.bits == 4 else "mxfp8"
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.ptrs = (k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr())
 
     @classmethod
@@ -656,14 +657,16 @@ class MXKV:
         """Streams [b0, b1) (views)."""
         return MXKV(self.k[b0:b1], self.k_scale[b0:b1], self.v[b0:b1], self.v_scale[b0:b1])
 
-    def _check(self, B, name, t):
-        """B streams with their int32 tensor `t`, on the current device."""
+    def _check(self, B, **tensors):
+        """B streams with their int32 tensors, on the current device."""
         if not 0 < B <= self.B:
             raise ValueError(f"{B} streams, the cache holds {self.B}")
-        if self.device.index != torch.cuda.current_device():
-            raise RuntimeError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        if t.dtype is not torch.int32 or t.numel() < B or not t.is_contiguous() or t.device != self.device:
-            raise ValueError(f"{name} must be a contiguous int32 tensor of {B} entries on {self.device}")
+        index = self.index
+        if index != _device():
+            raise RuntimeError(f"the cache is on {self.device}, the current device is cuda:{_device()}")
+        for name, t in tensors.items():
+            if t.dtype is not torch.int32 or t.numel() < B or not t.is_contiguous() or t.get_device() != index:
+                raise ValueError(f"{name} must be a contiguous int32 tensor of {B} entries on {self.device}")
 
     def _rows(self, x, name, n, ld, width):
         """Address of [n][ld] bf16 rows of which `width` elements are used: a raw device pointer (int) as it is, a
@@ -673,7 +676,7 @@ class MXKV:
         if isinstance(x, int):
             return x
         shape, strides = x.shape, x.stride()
-        if x.dtype is not torch.bfloat16 or x.device != self.device or len(shape) != 2 or strides[1] != 1:
+        if x.dtype is not torch.bfloat16 or x.get_device() != self.index or len(shape) != 2 or strides[1] != 1:
             raise ValueError(f"{name} must be a 2-dimensional bfloat16 tensor on {self.device} with unit element stride")
         if shape[0] < n or shape[1] < width or (n > 1 and strides[0] != ld):
             raise ValueError(f"{name}: {n} rows of {width} elements with stride {ld} from a tensor of shape "
@@ -684,7 +687,7 @@ class MXKV:
 def kv_append_mx(k_src, v_src, ld_k, ld_v, kv, pos0, B, n_new):
     """kv_append into a quantised cache: rows k_src/v_src [B*n_new][ld] bf16 (tensors or raw device pointers) into slots
     pos0[b] .. pos0[b] + n_new - 1 of stream b; slots outside the cache are skipped."""
-    kv._check(B, "pos0", pos0)
+    kv._check(B, pos0=pos0)
     w = kv.KVH * kv.D
     call("mgen_kv_append_mx", kv._rows(k_src, "k_src", B * n_new, ld_k, w), kv._rows(v_src, "v_src", B * n_new, ld_v, w),
          ld_k, ld_v, *kv.ptrs, pos0.data_ptr(), B, n_new, kv.KVH, kv.D, kv.max_len, kv.bits, _stream())
@@ -693,7 +696,7 @@ def kv_append_mx(k_src, v_src, ld_k, ld_v, kv, pos0, B, n_new):
 def kv_read_mx(kv, pos0, k_dst, v_dst, ld_k, ld_v, B, n):
     """The inverse of kv_append_mx: the values of slots pos0[b] .. pos0[b] + n - 1 into rows k_dst/v_dst [B*n][ld] bf16;
     rows whose slot is outside the cache stay as they were."""
-    kv._check(B, "pos0", pos0)
+    kv._check(B, pos0=pos0)
     w = kv.KVH * kv.D
     call("mgen_kv_read_mx", *kv.ptrs, pos0.data_ptr(), kv._rows(k_dst, "k_dst", B * n, ld_k, w),
          kv._rows(v_dst, "v_dst", B * n, ld_v, w), ld_k, ld_v, B, n, kv.KVH, kv.D, kv.max_len, kv.bits, _stream())
@@ -717,7 +720,7 @@ def _mx_workspace(workspace, kv, B, H, nsplit):
 def attn_decode_mx(q, ld_q, kv, kv_len, out, ld_o, workspace, B, H, nsplit, scale):
     """attn_decode over a quantised cache (an MXKV). q/out: rows [B][ld] bf16 (tensors or raw device pointers); a stream
     with kv_len[b] = 0 gets zeros, kv_len[b] beyond the cache counts as the cache's length."""
-    kv._check(B, "kv_len", kv_len)
+    kv._check(B, kv_len=kv_len)
     D = kv.D
     call("mgen_attn_decode_mx", kv._rows(q, "q", B, ld_q, H * D), ld_q, *kv.ptrs, kv_len.data_ptr(),
          kv._rows(out, "out", B, ld_o, H * D), ld_o, _mx_workspace(workspace, kv, B, H, nsplit), B, H, kv.KVH, D,
@@ -729,8 +732,7 @@ def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_le
     """attn_decode_prep over a quantised cache (an MXKV): q, new key and value from the raw projection rows, the new row
     quantised into slot pos[b] and attended. A stream whose pos[b] is no row of the cache or of the rotary table cs, or
     whose kv_len[b] is not pos[b] + 1, gets zeros and is not written."""
-    kv._check(B, "pos", pos)
-    kv._check(B, "kv_len", kv_len)
+    kv._check(B, pos=pos, kv_len=kv_len)
     D = kv.D
     for t, n, name in ((wq, D, "wq"), (wk, D, "wk"), (cs, D, "cs")):
         if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.device != kv.device or t.numel() < n):
@@ -743,8 +745,7 @@ def attn_decode_prep_mx(qkv, ld_in, wq, wk, cs, pos, eps, interleaved, kv, kv_le
 def decode_layer_mx(ptrs17, cs, pos, kv_len, kv, B, d, H, I, nsplit, eps, interleaved):
     """decode_layer over a quantised cache (an MXKV): ptrs17 as there; cs is the rotary table [positions, D/2, 2], pos and
     kv_len int32 tensors of at least B entries."""
-    kv._check(B, "pos", pos)
-    kv._check(B, "kv_len", kv_len)
+    kv._check(B, pos=pos, kv_len=kv_len)
     call("mgen_decode_layer_mx", *ptrs17, _p(cs), cs.shape[0], _p(pos), _p(kv_len), *kv.ptrs, B, d, H, kv.KVH, kv.D, I,
          kv.max_len, kv.bits, nsplit, eps, interleaved, _stream())
 

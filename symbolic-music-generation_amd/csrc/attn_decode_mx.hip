@@ -17,9 +17,10 @@
 // its own keys). Keys meet after the loop.
 //   256 streams x 8 heads x 128: 2048 keys in 8 bits 166 us (6.7 TB/s), 4096 in 4 bits 171 us (6.7), 2048 in 4 bits 91 (6.2).
 //
-// Several query heads (MXHeads), on the matrix cores: a unit of 32 keys goes from the loads' layout to the operands' through
-// LDS (as codes); lane (r, g), r = lane & 15, g = lane >> 4, then holds the g-th quarter of rows r and 16 + r, and its codes
-// become bf16 operand fragments of 8 elements (exactly).
+// Several query heads (MXHeads), on the matrix cores: units of 32 keys go straight to LDS, as codes, the next one on its way
+// while one is worked on (in registers 16 to 32 of them would hold it, and a CU the fewer waves); lane (r, g), r = lane & 15,
+// g = lane >> 4, takes the g-th quarter of rows r and 16 + r from there, and its codes become bf16 operand fragments of 8
+// elements (exactly).
 //  * Scores: the reduction runs over the elements in the order the lanes hold them, a permutation that q shares. The heads
 //    are the columns (columns i and 8 + i hold the same head): lane (r, g) ends up with column r, keys 4g .. 4g+3, which is
 //    the operand layout of the second product, so the weights never cross lanes.
@@ -30,7 +31,9 @@
 //    of weight at the price of 8); the two rows are added at the end.
 //  * A value block written with an infinity or a NaN enters as zeros and its elements of the result are set to NaN at the
 //    end (0 * NaN in the turning product would reach the other elements).
-//   256 streams x 8 kv heads of 4 x 128, 2048 keys in 4 bits 106 us (5.4 TB/s; a vector instruction mix of some 250 a unit).
+// The loads in flight bound it, the vector unit (250 instructions a unit) next to them. 256 streams x 8 kv heads x 128, 2048
+// keys in 4 bits: 102 us with 4 heads per kv head (5.6 TB/s); of 2 x 64: 59. 40 streams of 1 to 4000 keys, 8 kv heads of 4 x
+// 128, in 8 bits: 39 us (loads to registers, one unit at a time: 105, 67 and 51).
 //
 // Both: the running maximum of a head is shared by the wave and moves only when a score exceeds it by more than 2^8 in the
 // weight (sums stay far inside fp32); then the sums are scaled. Sums, maxima and outputs are fp32. Rows outside the split
@@ -38,6 +41,7 @@
 // and scale: the value 0), and the weights of the last unit of keys are masked.
 #include "kvmx.h"
 #include "decode_prep.h"
+#include "lds_dma.h"
 
 namespace {
 
@@ -82,13 +86,13 @@ __device__ __forceinline__ int mx_by_length(const int* kv_len, int max_len, int 
     float longest = 1.f;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        key[i] = -1;
-        if (i * 64 + lane < n) key[i] = max(min(kv_len[first + i * 64 + lane], max_len), 0);
+        key[i] = kv_len[first + min(i * 64 + lane, n - 1)];        // (without a branch: all of them under way together)
+        key[i] = max(min(key[i], max_len), 0);
         longest = fmaxf(longest, (float)key[i]);
     }
     const float unit = 255.9f / wave64_max(longest);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) key[i] = key[i] < 0 ? -1 : (int)((float)key[i] * unit);
+    for (int i = 0; i < NL; ++i) key[i] = i * 64 + lane < n ? (int)((float)key[i] * unit) : -1;
     int at = 0, above = 0;                // streams of key at or more: above rank; of more than that: `above`
 #pragma unroll 1
     for (int bit = 128; bit; bit >>= 1) {
@@ -126,6 +130,28 @@ __device__ __forceinline__ rsrc_t mx_rsrc(const unsigned char* p, unsigned bytes
 struct MXRsrc {                          // the split's keys: codes and scales of K and V
     rsrc_t k, ks, v, vs;
 };
+struct MXKeys {
+    const unsigned char *k, *ks, *v, *vs;
+};
+struct MXNew {                           // the step's own key, the last of the stream's last split
+    const bf16 *k, *v;                   // its rows in LDS
+    unsigned char *kc, *ks, *vc, *vs;    // their place in the cache
+    bool write, here;                    // this workgroup writes them; this split ends with it
+};
+// 16, 4 or 2 (zero-extended) bytes per lane from byte `from` of a buffer to 16 or 4 bytes per lane from LDS address dst on, past
+// the caches (read once: the non-temporal hint is worth 8 to 10 %); waited for by hand, see lds_dma.h
+template <int BYTES>
+__device__ __forceinline__ void mx_dma(const u32x4& rsrc, int from, unsigned dst) {
+    if (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                     : : "s"(dst), "v"(from), "s"(rsrc) : "memory", "m0");
+    else if (BYTES == 4)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                     : : "s"(dst), "v"(from), "s"(rsrc) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ushort %1, %2, 0 offen lds"
+                     : : "s"(dst), "v"(from), "s"(rsrc) : "memory", "m0");
+}
 __device__ __forceinline__ f32x4 mx_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -161,12 +187,11 @@ struct MXTiles {
             for (int i = 0; i < 4; ++i) c[t][i] = x[i];
         }
     }
-    // the codes of key t_new from its bf16 row, in the lanes that hold it; with `write` to the cache too (the row's codes
-    // and scale bytes). Returns the scale byte of the lane's block.
-    __device__ __forceinline__ static unsigned patch(unsigned (&c)[T][4], int t_new, int lane, const bf16* row, bool write,
-                                                     unsigned char* codes, unsigned char* scales) {
+    // the codes of the lane's elements of a bf16 row; with `write` to the cache too (the row's codes and scale bytes).
+    // Returns the scale byte of the lane's block.
+    __device__ __forceinline__ static unsigned encode(unsigned (&x)[4], int lane, const bf16* row, bool write,
+                                                      unsigned char* codes, unsigned char* scales) {
         const unsigned e = mx_block_exponent<BITS>(row, block(lane));
-        unsigned x[4];
 #pragma unroll
         for (int j = 0; j < ED / 8; ++j)
             mx_encode8<BITS>(*reinterpret_cast<const bf16x8*>(row + elem(lane) + 8 * j), e, x + j * WF);
@@ -174,10 +199,6 @@ struct MXTiles {
             *reinterpret_cast<u32x4*>(codes + lane % LR * 16) = u32x4{x[0], x[1], x[2], x[3]};
             scales[block(lane)] = (unsigned char)e;                 // (lanes of a block write the same byte)
         }
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[t][i] = t == t_new / KPT ? x[i] : c[t][i];
         return e;
     }
 };
@@ -190,7 +211,7 @@ struct MXOne {
     static constexpr int T = 4;
     typedef MXTiles<D, BITS, T> R;
     static constexpr int KPT = R::KPT, KPU = T * KPT, LR = R::LR, ED = R::ED, WF = R::WF, NB = R::NB;
-    static constexpr int IMG = 0;                     // bytes of LDS a wave works in
+    static constexpr int LDS = 0;                     // bytes of LDS a wave works in
     static constexpr int WAVES = 4;                   // a SIMD has to hold
     struct Unit {                                     // codes and scale bytes of K and of V
         unsigned k[T][4], v[T][4], ke[T], ve[T];
@@ -198,6 +219,7 @@ struct MXOne {
     bf16x2 q[ED / 2];
     float m, l, acc[ED], sl2;
     int lane;
+    MXRsrc src;                           // the split's codes and scales
 
     __device__ __forceinline__ void place(int lane_, char*) { lane = lane_; }
     __device__ __forceinline__ int key() const { return R::key(lane); }
@@ -216,9 +238,14 @@ struct MXOne {
     __device__ __forceinline__ void patch(unsigned (&c)[T][4], unsigned (&e)[T], int t_new, const bf16* row, bool write,
                                           unsigned char* codes, unsigned char* scales) const {
         if (key() != t_new % KPT) return;
-        const unsigned b = R::patch(c, t_new, lane, row, write, codes, scales);
+        unsigned x[4];
+        const unsigned b = R::encode(x, lane, row, write, codes, scales);
 #pragma unroll
-        for (int t = 0; t < T; ++t) e[t] = t == t_new / KPT ? b : e[t];
+        for (int t = 0; t < T; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[t][i] = t == t_new / KPT ? x[i] : c[t][i];
+            e[t] = t == t_new / KPT ? b : e[t];
+        }
     }
     __device__ __forceinline__ void start(const bf16* src, int nh, float scale_log2e) {
         sl2 = scale_log2e;
@@ -285,6 +312,26 @@ struct MXOne {
             }
         }
     }
+    __device__ __forceinline__ void begin(const MXKeys& keys, int, int n) {
+        src = {mx_rsrc(keys.k, n * R::RB), mx_rsrc(keys.ks, n * NB), mx_rsrc(keys.v, n * R::RB), mx_rsrc(keys.vs, n * NB)};
+    }
+    template <int NW>
+    __device__ __forceinline__ void walk(int base, int n, const MXNew& fresh) {
+        Unit u;
+#pragma unroll 1
+        for (; base + KPU < n; base += NW * KPU) {   // units before the one with the split's last key
+            load(src, base, u);
+            unit<false>(u, 0);
+        }
+        if (base < n) {
+            load(src, base, u);
+            if (fresh.here) {
+                patch(u.k, u.ke, n - 1 - base, fresh.k, fresh.write, fresh.kc, fresh.ks);
+                patch(u.v, u.ve, n - 1 - base, fresh.v, fresh.write, fresh.vc, fresh.vs);
+            }
+            unit<true>(u, n - base);
+        }
+    }
     // The wave's maximum, denominator and sums to ml[2] and o[D]. Lanes that hold the same elements (64 / LR keys) add up,
     // halving the elements a lane is responsible for at every step: a swap of half waves or of neighbouring rows of 16
     // lanes brings two elements' halves together, then exchanges inside a row.
@@ -328,77 +375,111 @@ struct MXOne {
 template <int D, int BITS>
 struct MXHeads {
     static constexpr int RB = MX<D, BITS>::RB, NB = MX<D, BITS>::NB;
-    static constexpr int KPU = 32, T = KPU / MXTiles<D, BITS, 1>::KPT;
-    typedef MXTiles<D, BITS, T> R;
+    static constexpr int KPU = 32;
+    typedef MXTiles<D, BITS, 1> R;
+    static constexpr int T = KPU / R::KPT;            // loads of a unit's codes of K (of V)
     static constexpr int W = RB / 16;                 // dwords of a quarter row
     static constexpr int NF = D / 32;                 // fragments of 8 elements
     static constexpr int WF = BITS / 4;               // dwords of a fragment
-    static constexpr int IMG = KPU * RB;              // bytes of LDS a wave works in: the codes of a unit
-    static constexpr int WAVES = RB == 128 ? 3 : 4;   // a SIMD has to hold (more registers than 4 leave where T is 4)
-    struct Unit {                                     // codes as they were loaded; scale bytes of a lane's quarter rows
-        unsigned k[T][4], v[T][4], ke[2], ve[2];
-    };
+    // a unit in LDS: codes of K and of V, a dword of scale bytes per key of K and of V; two a wave, one of them ahead
+    static constexpr int IMG = KPU * RB, SLOT = 2 * IMG + 2 * 4 * KPU, LOADS = 2 * T + 2;
+    static constexpr int LDS = 2 * SLOT;              // bytes of LDS a wave works in
+    static constexpr int WAVES = RB == 128 ? 2 : 3;   // a SIMD has to hold (what LDS leaves)
     bf16x8 qf[NF], pick[2];
     float m, l, sl2, low;                 // of column r; low: the column takes the weights' remainders
     f32x4 acc[NF][2];                     // rows = columns of the scores, column r of selection c
     unsigned long long bad;               // lanes that met a value block of scale 255
     char* img;
     int lane, r, g;
+    u32x4 rk, rks, rv, rvs;               // the split's codes and scales
+    unsigned lds;                         // address of the wave's slots
 
     __device__ __forceinline__ void place(int lane_, char* image) {
         lane = lane_;
         r = lane & 15;
         g = lane >> 4;
         img = image;
+        lds = __builtin_amdgcn_readfirstlane(lds_addr(image));
     }
     __device__ __forceinline__ static int elem_of(int j, int g) { return g * (D / 4) + 8 * j; }
     __device__ __forceinline__ int elem(int j) const { return elem_of(j, g); }
     __device__ __forceinline__ int block() const { return g * NB / 4; }
-
-    __device__ __forceinline__ void load(const MXRsrc& s, int base, Unit& u) const {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int at = (base + 16 * t + r) * NB + block();
-            u.ke[t] = __builtin_amdgcn_raw_buffer_load_b8(s.ks, at, 0, 0);
-            u.ve[t] = __builtin_amdgcn_raw_buffer_load_b8(s.vs, at, 0, 0);
-        }
-        R::template load<2>(s.k, base, lane, u.k);
-        R::template load<2>(s.v, base, lane, u.v);
-    }
-    __device__ __forceinline__ void patch(unsigned (&c)[T][4], unsigned (&e)[2], int t_new, const bf16* row, bool write,
-                                          unsigned char* codes, unsigned char* scales) const {
-        if (R::key(lane) == t_new % R::KPT) R::patch(c, t_new, lane, row, write, codes, scales);
-        if (r == (t_new & 15)) {
-            const unsigned b = mx_block_exponent<BITS>(row, block());
-#pragma unroll
-            for (int t = 0; t < 2; ++t) e[t] = t == t_new >> 4 ? b : e[t];
-        }
-    }
     // 16-byte chunk c of a row of the image, spread so that 16 rows' chunks lie on different banks
     __device__ __forceinline__ static int at(int row, int c) {
         return row * RB + 16 * (c ^ (RB == 128 ? row >> 1 & 7 : RB == 64 ? row >> 2 & 3 : row >> 3 & 1));
     }
-    // from the loads' layout to the lane's quarters of key r of both tiles, through the wave's image
-    __device__ __forceinline__ void spread(const unsigned (&c)[T][4], unsigned (&out)[2][W]) {
+
+    // unit [base, base + KPU) of the split on its way to a slot: each load a contiguous kilobyte, its chunks in the order of
+    // the image; rows behind the split's last key arrive as zeros
+    __device__ __forceinline__ void request(int base, int slot) const {
+        const unsigned dst = lds + slot * SLOT;
+        const int row = R::key(lane), c = lane % R::LR;
 #pragma unroll
-        for (int t = 0; t < T; ++t)
-            lds_write_b128(img, at(t * R::KPT + R::key(lane), lane % R::LR), u32x4{c[t][0], c[t][1], c[t][2], c[t][3]});
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int row = 16 * t + r;
-            if (W == 2) {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(img + at(row, g >> 1) + 8 * (g & 1));
-                out[t][0] = x[0];
-                out[t][1] = x[1];
-            } else {
-#pragma unroll
-                for (int h = 0; h < W / 4; ++h) {
-                    const u32x4 x = *reinterpret_cast<const u32x4*>(img + at(row, g * (W / 4) + h));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) out[t][4 * h + i] = x[i];
+        for (int t = 0; t < T; ++t) {
+            const int from = (base + t * R::KPT + row) * RB + (at(t * R::KPT + row, c) & (RB - 1));
+            mx_dma<16>(rk, from, dst + t * 1024);
+            mx_dma<16>(rv, from, dst + IMG + t * 1024);
+        }
+        if (lane < KPU) {
+            mx_dma<NB>(rks, (base + lane) * NB, dst + 2 * IMG);
+            mx_dma<NB>(rvs, (base + lane) * NB, dst + 2 * IMG + 4 * KPU);
+        }
+    }
+    __device__ __forceinline__ void begin(const MXKeys& keys, int base, int n) {
+        rk = dma_rsrc(keys.k, n * RB);
+        rks = dma_rsrc(keys.ks, n * NB);
+        rv = dma_rsrc(keys.v, n * RB);
+        rvs = dma_rsrc(keys.vs, n * NB);
+        if (base < n) request(base, 0);
+    }
+    template <int NW>
+    __device__ __forceinline__ void walk(int base, int n, const MXNew& fresh) {
+        int slot = 0;
+#pragma unroll 1
+        for (; base < n; base += NW * KPU, slot ^= 1) {
+            if (base + NW * KPU < n) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read from the slot that is filled again
+                request(base + NW * KPU, slot ^ 1);
+                dma_wait<LOADS>();
+            } else dma_wait<0>();
+            const int left = n - base;
+            char* here = img + slot * SLOT;
+            if (left > KPU) unit<false>(here, 0);
+            else {
+                if (fresh.here) {
+                    patch(here, 0, left - 1, fresh.k, fresh.write, fresh.kc, fresh.ks);
+                    patch(here, 1, left - 1, fresh.v, fresh.write, fresh.vc, fresh.vs);
                 }
+                unit<true>(here, left);
             }
         }
+    }
+    // key t_new of a unit, K (value = 0) or V, from its bf16 row
+    __device__ __forceinline__ void patch(char* unit, int value, int t_new, const bf16* row, bool write,
+                                          unsigned char* codes, unsigned char* scales) const {
+        if (lane >= R::LR) return;
+        unsigned x[4];
+        const unsigned e = R::encode(x, lane, row, write, codes, scales);
+        lds_write_b128(unit + value * IMG, at(t_new, lane), u32x4{x[0], x[1], x[2], x[3]});
+        unit[2 * IMG + (value * KPU + t_new) * 4 + R::block(lane)] = (char)e;
+    }
+    // the lane's quarter of key 16 t + r, and its block's scale byte
+    __device__ __forceinline__ unsigned quarter(const char* unit, int value, int t, unsigned (&out)[W]) const {
+        const char* image = unit + value * IMG;
+        const int row = 16 * t + r;
+        if (W == 2) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(image + at(row, g >> 1) + 8 * (g & 1));
+            out[0] = x[0];
+            out[1] = x[1];
+        } else {
+#pragma unroll
+            for (int h = 0; h < W / 4; ++h) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(image + at(row, g * (W / 4) + h));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[4 * h + i] = x[i];
+            }
+        }
+        return *reinterpret_cast<const unsigned char*>(unit + 2 * IMG + (value * KPU + row) * 4 + block());
     }
 
     __device__ __forceinline__ void start(const bf16* q, int nh, float scale_log2e) {
@@ -423,15 +504,16 @@ struct MXHeads {
             for (int c = 0; c < 2; ++c) acc[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     template <bool LAST>
-    __device__ __forceinline__ void unit(const Unit& u, int left) {
+    __device__ __forceinline__ void unit(const char* slot, int left) {
         float s[8];
-        unsigned c[2][W];
-        spread(u.k, c);
+        unsigned c[2][W], e[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) e[t] = quarter(slot, 0, t, c[t]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < NF; ++j) a = mx_mfma(mx_decode8<BITS>(c[t] + j * WF, mx_scale(u.ke[t])), qf[j], a);
+            for (int j = 0; j < NF; ++j) a = mx_mfma(mx_decode8<BITS>(c[t] + j * WF, mx_scale(e[t])), qf[j], a);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[4 * t + i] = a[i] * sl2;
@@ -465,12 +547,12 @@ struct MXHeads {
             l += w;
             p[i] = (bf16)fmaf(-low, round_bf(w), w);
         }
-        spread(u.v, c);
         float vs[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            bad |= __ballot(u.ve[t] == 255u);
-            vs[t] = u.ve[t] == 255u ? 0.f : mx_scale(u.ve[t]);
+            e[t] = quarter(slot, 1, t, c[t]);
+            bad |= __ballot(e[t] == 255u);
+            vs[t] = e[t] == 255u ? 0.f : mx_scale(e[t]);
         }
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
@@ -532,12 +614,12 @@ __global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_m
                                                                     threadIdx.x & 63));
     const int h0 = kvh * group + chunk * MX_HEADS, nh = min(MX_HEADS, group - chunk * MX_HEADS), hc = min(MX_HEADS, group);
     // LDS: q heads, new key and new value (PREP) and what the cores work in, which then give way to the waves' sums
-    bf16* sm_q = reinterpret_cast<bf16*>(smem + NW * C::IMG / 4);    // [hc + 2][D]
+    bf16* sm_q = reinterpret_cast<bf16*>(smem + NW * C::LDS / 4);    // [hc + 2][D]
     float* sm_o = smem;                              // [NW][hc][D]
     float* sm_ml = smem + NW * hc * D;               // [NW][hc][2]
     const int tid = threadIdx.x, wave = tid >> 6;
     C core;
-    core.place(tid & 63, reinterpret_cast<char*>(smem) + wave * C::IMG);
+    core.place(tid & 63, reinterpret_cast<char*>(smem) + wave * C::LDS);
 
     const int len = mx_length<PREP>(kv_len, kv.max_len, pp, b), pos = len - 1;       // (pos: of the new token, PREP)
     if (len <= 0) {                       // a stream without keys: zeros
@@ -551,12 +633,10 @@ __global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_m
     if (n <= 0) return;
 
     const long slice = ((long)b * KVH + kvh) * kv.max_len;
-    const unsigned nk = (unsigned)n;
-    const MXRsrc src{mx_rsrc(kv.k + (slice + k_beg) * RB, nk * RB), mx_rsrc(kv.ks + (slice + k_beg) * NB, nk * NB),
-                     mx_rsrc(kv.v + (slice + k_beg) * RB, nk * RB), mx_rsrc(kv.vs + (slice + k_beg) * NB, nk * NB)};
-
-    int base = wave * KPU;
-    typename C::Unit u;
+    const long first_row = slice + k_beg;
+    const MXKeys keys{kv.k + first_row * RB, kv.ks + first_row * NB, kv.v + first_row * RB, kv.vs + first_row * NB};
+    const int base = wave * KPU;
+    core.begin(keys, base, n);
 
     if (PREP) {
         constexpr int L16 = D / 16;
@@ -579,26 +659,19 @@ __global__ __launch_bounds__(64 * NW, (Core<D, BITS>::WAVES)) void attn_decode_m
         __syncthreads();
     }
     core.start(PREP ? sm_q : q + (long)b * ld_q + (long)h0 * D, nh, scale * MX_LOG2E);
+    // q has arrived before the walk: the compiler would wait for it inside, and with it for the units that are under way
+    if (C::LDS) __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0)
 
-#pragma unroll 1
-    for (; base + KPU < n; base += NW * KPU) {       // units before the one with the split's last key
-        core.load(src, base, u);
-        core.template unit<false>(u, 0);
+    MXNew fresh{};
+    if (PREP) {
+        const long at = slice + pos;
+        fresh = {sm_q + hc * D, sm_q + (hc + 1) * D, const_cast<unsigned char*>(kv.k) + at * RB,
+                 const_cast<unsigned char*>(kv.ks) + at * NB, const_cast<unsigned char*>(kv.v) + at * RB,
+                 const_cast<unsigned char*>(kv.vs) + at * NB, chunk == 0, k_beg + n == len};
     }
-    if (base < n) {
-        core.load(src, base, u);
-        const int t_new = n - 1 - base;   // the stream's last key, in its last split
-        if (PREP && k_beg + n == len) {
-            const long at = slice + pos;
-            core.patch(u.k, u.ke, t_new, sm_q + hc * D, chunk == 0, const_cast<unsigned char*>(kv.k) + at * RB,
-                       const_cast<unsigned char*>(kv.ks) + at * NB);
-            core.patch(u.v, u.ve, t_new, sm_q + (hc + 1) * D, chunk == 0, const_cast<unsigned char*>(kv.v) + at * RB,
-                       const_cast<unsigned char*>(kv.vs) + at * NB);
-        }
-        core.template unit<true>(u, n - base);
-    }
+    core.template walk<NW>(base, n, fresh);
 
-    if (PREP || C::IMG) __syncthreads();  // the sums overwrite both
+    if (PREP || C::LDS) __syncthreads();  // the sums overwrite both
     core.finish(sm_ml + wave * hc * 2, sm_o + wave * hc * D, nh);
     __syncthreads();
 #pragma unroll 1
@@ -681,12 +754,12 @@ __global__ __launch_bounds__(256) void attn_decode_mx_merge_kernel(const float* 
 }
 
 template <int D, int BITS, int PREP, template <int, int> class Core, int NW>
-void launch(const void* q, long ld_q, MXView kv, const int* kv_len, void* out, long ld_o, float* ws, int B, int H,
+int launch(const char* what, const void* q, long ld_q, MXView kv, const int* kv_len, void* out, long ld_o, float* ws, int B, int H,
             int KVH, int nsplit, float scale, MXPrep pp, hipStream_t stream) {
     float* part_ml = ws;
     float* part_o = ws ? ws + (long)B * H * nsplit * 2 : nullptr;
     const int group = H / KVH, chunks = (group + MX_HEADS - 1) / MX_HEADS, hc = group < MX_HEADS ? group : MX_HEADS;
-    const int loop = NW * Core<D, BITS>::IMG + (PREP ? (hc + 2) * D * 2 : 0), sums = NW * hc * (D + 2) * 4;
+    const int loop = NW * Core<D, BITS>::LDS + (PREP ? (hc + 2) * D * 2 : 0), sums = NW * hc * (D + 2) * 4;
     const int lds = loop > sums ? loop : sums;
     // More workgroups than the chip holds: behind the streams that start at once (their order does not matter, and it would
     // show as latency) the longest go first, or a long one that starts last runs on alone. 256 x 8 heads x 128, lengths up
@@ -694,12 +767,28 @@ void launch(const void* q, long ld_q, MXView kv, const int* kv_len, void* out, l
     // and 108; equal lengths 168 and 169. Short caches end before it pays (96 x 24 heads, 3 keys: 14.0 and 17.5).
     const long groups = (long)KVH * chunks * nsplit, at_once = MX_PLACES / groups;
     const int first = kv.max_len >= MX_ORDER_KEYS && B > at_once && B - at_once <= MX_ORDERED ? (int)at_once : B;
+    if (lds > 65536) {                    // more than the default 64 KiB of dynamic LDS: asked for once per kernel and device
+        static bool asked[64] = {};
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        dev = dev < 0 || dev > 63 ? 63 : dev;
+        if (!asked[dev]) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_decode_mx_kernel<D, BITS, PREP, Core, NW>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+            if (e != hipSuccess) {
+                mgen_set_error("%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
+                return MGEN_ELAUNCH;
+            }
+            asked[dev] = true;
+        }
+    }
     hipLaunchKernelGGL((attn_decode_mx_kernel<D, BITS, PREP, Core, NW>), dim3(nsplit, KVH * chunks, B), dim3(64 * NW), lds,
                        stream, (const bf16*)q, ld_q, kv, kv_len, H, KVH, nsplit, first, scale, part_ml, part_o, (bf16*)out, ld_o,
                        pp);
     if (nsplit > 1)
         hipLaunchKernelGGL((attn_decode_mx_merge_kernel<D, PREP>), dim3(H, B), dim3(256), 0, stream, part_ml, part_o, kv_len,
                            kv.max_len, pp, nsplit, H, (bf16*)out, ld_o);
+    return mgen_check_launch(what);
 }
 
 template <int PREP>
@@ -720,28 +809,32 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
     MGEN_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (D / 32 - 1)) == 0, "%s: scales must be aligned to a row (D / 32)", what);
     const MXView kv{(const unsigned char*)kc, (const unsigned char*)ks, (const unsigned char*)vc,
                     (const unsigned char*)vs, max_len};
-    // Several heads: 8 waves where a CU gets one workgroup or none (1 stream of 100003 keys, 4 kv heads of 4, 64 splits: 25 us
-    // against 29 in workgroups of 4; 32 x 8 kv heads of 8, 4096 keys: 48 and 54), 4 beyond (96 x 24, 3 keys: 27 and 14).
+    // Several heads: 8 waves where a CU gets one workgroup or none (with loads to registers: 1 stream of 100003 keys, 4 kv heads
+    // of 4, 64 splits 25 us against 29 in workgroups of 4; 32 x 8 kv heads of 8, 4096 keys 48 and 54), 4 beyond (96 x 24, 3 keys:
+    // 27 and 14).
 #define LAUNCH(DD, BB)                                                                                                 \
     do {                                                                                                               \
-        if (H == KVH) launch<DD, BB, PREP, MXOne, 4>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
-        else if ((long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS) * nsplit <= 256)                                \
-            launch<DD, BB, PREP, MXHeads, 8>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
-        else launch<DD, BB, PREP, MXHeads, 4>(q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream);  \
+        if (H == KVH)                                                                                                  \
+            return launch<DD, BB, PREP, MXOne, 4>(what, q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
+        if ((long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS) * nsplit <= 256)                                     \
+            return launch<DD, BB, PREP, MXHeads, 8>(what, q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream); \
+        return launch<DD, BB, PREP, MXHeads, 4>(what, q, ld_q, kv, kv_len, out, ld_o, ws, B, H, KVH, nsplit, scale, pp, stream);  \
     } while (0)
     if (D == 128) { if (bits == 4) LAUNCH(128, 4); else LAUNCH(128, 8); }
-    else { if (bits == 4) LAUNCH(64, 4); else LAUNCH(64, 8); }
+    if (bits == 4) LAUNCH(64, 4);
+    LAUNCH(64, 8);
 #undef LAUNCH
-    return mgen_check_launch(what);
 }
 
 }  // namespace
 
 // Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
-// Few workgroups: as many splits as bring them to 512 (several heads: 1024), each with keys for two rounds of its waves or
-// more, where the second launch is worth its 3 us: from 8 rounds on (1 stream x 8 heads x 128 in 8 bits: 4096 keys, 32
-// rounds, 33 us in one split and 8.3 in 16; 512 keys, 4 rounds, 5.7 and 7.6. 16 streams of up to 8192 keys, 8 kv heads of
-// 4: 27 us in 4 splits, 24 in 8).
+// Few workgroups: a power of two of splits (the chip's places divide evenly) that brings them to 512, to 1280 while each has
+// 1024 keys, and never less than two rounds of keys for a workgroup's waves; where the second launch is worth its 3 us, from
+// 8 rounds on. Measured, us: 1 stream x 8 heads x 128 in 8 bits, 4096 keys 33 in one split and 8.3 in 16, 512 keys 5.7 and
+// 7.6. 16 streams of 8 kv heads x 128 of up to 6000 keys, 4 heads each, 4 / 8 bits: 20.7 / 29.9 in 4 splits, 20.3 / 34.9 in
+// 6, 21.3 / 34.6 in 8; up to 32768 keys 79 / 119, 62 / 122, 59 / 116. 24 streams of up to 6000 keys, one head each, 26.5 / 38.7
+// in 2 splits, 19.8 / 33.7 in 4.
 // From 256 workgroups on: one (two, at 1500 keys: 1536 workgroups of heads of 64 in 4 bits 28 and 38 us, in 8 bits 50 and 52,
 // of 128 96 and 99; at 6000 keys 347 and 355).
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
@@ -749,10 +842,11 @@ extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int long
     const bool one = H == KVH;
     const long groups = (long)B * KVH * ((H / KVH + MX_HEADS - 1) / MX_HEADS);
     const int round = one && D == 64 ? 256 : 128;     // keys of a round of a workgroup's waves, taken at 8 bits
-    const int rounds = (longest + round - 1) / round;
+    const int rounds = (longest - 1) / round + 1;
     if (rounds < 8 || groups >= 256) return 1;
-    const long n = (one ? 512 : 1024) / groups, most = rounds / 2;
-    return (int)(n < most ? (n < MX_MAX_SPLITS ? n : MX_MAX_SPLITS) : most < MX_MAX_SPLITS ? most : MX_MAX_SPLITS);
+    int n = MX_MAX_SPLITS;
+    while (n > 1 && (n * groups > 1280 || (n * groups > 512 && longest < 1024 * n))) n /= 2;
+    return n < rounds / 2 ? n : rounds / 2;
 }
 
 // q [B][ld_q] (heads at h*D), out [B][ld_o] bf16; kv_len[b] = cached keys of stream b (0: the output row is zeros; values

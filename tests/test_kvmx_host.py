@@ -100,3 +100,15 @@ def test_cache_object_refuses():
             ops.MXKV(u8(1, 1, 4, w), u8(1, 1, 4, d // 32), u8(1, 1, 4, w), u8(1, 1, 4, d // 32))
     with pytest.raises(ValueError, match="mxfp6"):
         ops.MXKV.empty(1, 1, 4, 64, "mxfp6", "cpu")
+
+
+@pytest.mark.parametrize("B,H,KVH,D", [(1, 8, 8, 128), (3, 24, 24, 64), (16, 32, 8, 128), (24, 8, 8, 128), (28, 64, 8, 64),
+                                       (31, 8, 8, 64), (32, 8, 8, 128), (200, 12, 1, 64), (255, 1, 1, 128), (300, 4, 4, 64)])
+def test_suggested_splits_never_fall_with_the_length(B, H, KVH, D):
+    """A workspace sized for the longest call of a run holds all of them."""
+    from mgen import ops
+    last = 0
+    for longest in [*range(1, 3000, 37), *range(3000, 140000, 1021), 1 << 24, (1 << 31) - 1]:
+        n = ops.attn_decode_mx_splits(B, H, KVH, D, longest)
+        assert 1 <= n <= 64 and n >= last
+        last = n

@@ -183,21 +183,21 @@ struct TileStream {
     // (scalar); wave = this wave's (scalar) index. An asm statement: the compiler does not know that an LDS write is
     // pending (it would drain it with s_waitcnt vmcnt(0) in front of the next transposed LDS read, in the middle of
     // the tile the prefetch is meant to overlap). The caller waits (asm s_waitcnt vmcnt) and passes a barrier before
-    // anyone reads the image. M0 (the instruction's LDS base) is saved and restored.
+    // anyone reads the image.
     // extra = a byte offset inside the token row (another head of the row the descriptor starts at)
     __device__ __forceinline__ void issue_piece(int j, int row0, unsigned lds_base, int wave, int extra = 0) const {
-        unsigned keep;
         const unsigned dst = __builtin_amdgcn_readfirstlane(lds_base + (unsigned)(wave + NW * j) * 1024u);
         const int soff = __builtin_amdgcn_readfirstlane((row0 + 4 * NW * j) * row_bytes + extra);
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
-                     "buffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-                     : "=&s"(keep) : "s"(dst), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+        // s_nop 3: a load may read a scalar register five wait states after the vector ALU wrote it (v_readlane of a
+        // spilled soff stands right before this statement in the forward kernel; tools/audit_asm_waits.py)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     : : "s"(dst), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
     }
     __device__ __forceinline__ void issue(int row0, unsigned lds_base, int wave, int extra = 0) const {
 #pragma unroll
         for (int j = 0; j < NP; ++j) issue_piece(j, row0, lds_base, wave, extra);
     }
-    // the same piece with M0 declared clobbered instead of saved and restored (kernels that never rely on M0)
+    // the same piece for the dK/dV kernel, whose scalar offsets are never spilled (the build's audit checks the distance)
     __device__ __forceinline__ void issue_piece_m0(int j, int row0, unsigned lds_base, int wave, int extra = 0) const {
         const unsigned dst = __builtin_amdgcn_readfirstlane(lds_base + (unsigned)(wave + NW * j) * 1024u);
         const int soff = __builtin_amdgcn_readfirstlane((row0 + 4 * NW * j) * row_bytes + extra);

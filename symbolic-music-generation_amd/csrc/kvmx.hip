@@ -129,8 +129,9 @@ int rows_of(const char* what, const void* k, const void* v, const void* kc, cons
     MGEN_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (D / 32 - 1)) == 0, "%s: scales must be aligned to a row (D / 32)", what);
     int shift = 0;              // a tile: at most the rows of a workgroup, no more than the tokens need
     while ((1 << shift) < 2048 / D && (1 << shift) < n) ++shift;
-    const long tiles = ((long)n + (1 << shift) - 1) >> shift, rows = (B * tiles * KVH) << shift;
-    MGEN_REQUIRE(rows < (1l << 31), "%s: too many rows (%ld)", what, rows);
+    const long tiles = ((long)n + (1 << shift) - 1) >> shift, per_stream = (tiles << shift) * KVH;      // (below 2^63)
+    MGEN_REQUIRE(per_stream < (1l << 31) && B * per_stream < (1l << 31), "%s: too many rows (B=%d n=%d KVH=%d)", what, B, n, KVH);
+    const long rows = B * per_stream;
     *a = {fast_div((unsigned)tiles), fast_div((unsigned)KVH), (unsigned)rows, (unsigned)n, shift, max_len, pos0};
     return MGEN_OK;
 }

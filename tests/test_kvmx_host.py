@@ -112,3 +112,14 @@ def test_suggested_splits_never_fall_with_the_length(B, H, KVH, D):
         n = ops.attn_decode_mx_splits(B, H, KVH, D, longest)
         assert 1 <= n <= 64 and n >= last
         last = n
+
+
+@pytest.mark.parametrize("fn,args", [("mgen_kv_append_mx", _append), ("mgen_kv_read_mx", _read)])
+@pytest.mark.parametrize("big", [dict(B=1 << 30, n=1 << 30, KVH=1 << 8, ldk=1 << 15, ldv=1 << 15),
+                                 dict(B=(1 << 31) - 1, n=(1 << 31) - 1, KVH=(1 << 31) - 1, ldk=1 << 40, ldv=1 << 40),
+                                 dict(B=1 << 16, n=1 << 15)], ids=str)
+def test_row_counts_do_not_wrap(fn, args, big):
+    """2^64 rows are 0 in 64 bits: refused as too many, not launched as none."""
+    from mgen._lib import MgenError, call
+    with pytest.raises(MgenError, match="too many rows"):
+        call(fn, *args(**big))

@@ -57,6 +57,8 @@ def attend(q, k, v, scale):
     the exponential of a difference whose log2 is off by its own rounding (|s| 2^-24 each way, |s| <= S), plus n 2^-24 for
     each of the two sums over the keys; weights enter numerator and denominator: twice, on sum_j p_j |v_j|. The split of
     the keys adds one rounding a split (at most 64).
+    With several query heads a kv head a weight w in [1, 2) enters the numerator as two bf16 numbers: the first is off by at
+    most 2^-8, so what it leaves is at most that and the second is off by at most 2^-17 (half a step below 2^-8): that once.
     Weights are taken against a maximum that may lag the true one by 2^8 and are lost below fp32's smallest normal number
     (so are the factors that join waves and splits, each on a sum of at most n weights of at most 2^8), while the
     denominator is at least 1: n 2^8 2^-126 max_j |v_j| twice."""
@@ -73,5 +75,7 @@ def attend(q, k, v, scale):
         out[h] = p @ vv
         S = scale * (np.abs(kk) @ np.abs(q[h])).max()
         rel = (D + 4) * 2.0 ** -24 * S + 2 * S * 2.0 ** -24 + 2.0 ** -21 + (n + 64) * 2.0 ** -24
-        bound[h] = 2.0 ** -8 * np.abs(out[h]) + 2 * rel * (p @ np.abs(vv)) + n * 2.0 ** -117 * np.abs(vv).max(0)
+        two = 2.0 ** -17 if H > kvh else 0.0
+        bound[h] = (2.0 ** -8 * np.abs(out[h]) + (2 * rel + two) * (p @ np.abs(vv))
+                    + n * 2.0 ** -117 * np.abs(vv).max(0))
     return out, bound

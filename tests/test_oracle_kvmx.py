@@ -68,3 +68,16 @@ def test_attention_of_one_key_is_its_value_and_of_none_zero():
 def test_no_rows(fmt):
     code, e = K.quantise(np.zeros((2, 0, 64)), fmt)
     assert code.shape == (2, 0, 64) and e.shape == (2, 0, 2) and K.values(K.pack(code, fmt), e, fmt).shape == (2, 0, 64)
+
+
+def test_weights_in_two_bf16_numbers():
+    """What the bound of several query heads a kv head counts for them, and that it is not idle."""
+    import torch
+    w = 1 + torch.rand(1 << 20, generator=torch.Generator().manual_seed(0))
+    w = torch.cat([w, 1 + 2.0 ** -8 - torch.arange(1, 1 << 15) * 2.0 ** -23])
+    high = w.bfloat16().float()
+    off = ((high + (w - high).bfloat16().float()).double() - w.double()).abs()
+    assert 2.0 ** -18 < float(off.max()) <= 2.0 ** -17
+    q, k, v = np.zeros((2, 64)), np.zeros((1, 1, 64)), np.ones((1, 1, 64))
+    several, one = K.attend(q, k, v, 1.0)[1], K.attend(q[:1], k, v, 1.0)[1]
+    assert np.allclose(several - one, 2.0 ** -17, rtol=1e-6)

@@ -431,7 +431,8 @@ int mgen_kv_read_mx(const void* k_codes, const void* k_scales, const void* v_cod
                     int max_len, int bits, mgen_stream_t stream);
 /* mgen_attn_decode over that cache (TF models/qwen3/modeling_qwen3.py:259-279 with q_len = 1): softmax statistics, weights
  * and sums in fp32. kv_len[b] = keys of stream b: 0 (or less) gives an output row of zeros, more than max_len counts as
- * max_len. nsplit (1 .. 64) workgroups share a stream's keys; mgen_attn_decode_mx_splits suggests a count for calls whose
+ * max_len. Results are finite while the magnitude of the scores stays below 2^100 and that of the values below 2^119 / keys.
+ * nsplit (1 .. 64) workgroups share a stream's keys; mgen_attn_decode_mx_splits suggests a count for calls whose
  * longest stream has `longest` keys; nsplit > 1 needs mgen_attn_decode_workspace(B, H, D, nsplit) floats. */
 int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest);
 int mgen_attn_decode_mx(const void* q, long ld_q, const void* k_codes, const void* k_scales, const void* v_codes,

@@ -10,12 +10,13 @@
 //
 // One workgroup per (key split, kv head with up to 8 query heads, stream); its waves walk units of keys. A load instruction
 // is one contiguous kilobyte of codes (MXTiles). Streams of different lengths: 256 x 8 heads x 128, 1 to 4096 keys in 4 bits
-// 97 us (6.0 TB/s; the same number of keys in equal streams 93).
+// 92 to 97 us (6.1 TB/s; as many keys in equal streams 91 to 98).
 //
 // One query head per kv head (MXOne), all on the vector unit. Scores: codes to bf16 pairs, two products and their sum per
 // instruction, the 2, 4 or 8 lanes of a row add up. V: codes to fp32, weighted into the lane's own sums (its elements, over
 // its own keys). Keys meet after the loop.
-//   256 streams x 8 heads x 128: 2048 keys in 8 bits 166 us (6.7 TB/s), 4096 in 4 bits 171 us (6.7), 2048 in 4 bits 91 (6.2).
+//   256 streams x 8 heads x 128: 2048 keys in 8 bits 163 us (6.8 TB/s), 4096 in 4 bits 170 to 189 by where its buffers lie
+//   (6.7 to 6.1), 2048 in 4 bits 91 to 98 (6.2 to 5.8).
 //
 // Several query heads (MXHeads), on the matrix cores: units of 32 keys go straight to LDS, as codes, the next one on its way
 // while one is worked on (in registers 16 to 32 of them would hold it, and a CU the fewer waves); lane (r, g), r = lane & 15,
@@ -33,12 +34,16 @@
 //    of weight at the price of 8); the two rows are added at the end.
 //  * A value block written with an infinity or a NaN enters as zeros and its elements of the result are set to NaN at the
 //    end (0 * NaN in the turning product would reach the other elements).
-// The loads in flight bound it, the vector unit (250 instructions a unit) next to them. 256 streams x 8 kv heads x 128, 2048
-// keys in 4 bits: 102 us with 4 heads per kv head (5.6 TB/s); of 2 x 64: 59. 40 streams of 1 to 4000 keys, 8 kv heads of 4 x
-// 128, in 8 bits: 39 us (loads to registers, one unit at a time: 105, 67 and 51).
+// Bound on a full chip: in 4 bits the vector unit (250 instructions a unit: 74 % busy, the matrix pipe 35 %; a wave waits
+// for its turn to issue 44 % of its time, for data 27 %), in 8 bits HBM (6.8 TB/s at 128 x 8192 keys with 4 heads per kv head;
+// vector unit 42 %). Fewer but slower instructions in its place gave nothing: a unit is one dependent chain (scores, weights,
+// turn, rounding, product), which is also what few streams of unequal lengths wait for. 256 streams x 8 kv heads x 128, 2048
+// keys in 4 bits: 102 us with 4 heads per kv head (5.6 TB/s); of 2 x 64: 58. 40 streams of 1 to 4000 keys, 8 kv heads of 4 x
+// 128, in 8 bits: 37 to 39 us (loads to registers, one unit at a time: 105, 67 and 51).
 //
 // Both: the running maximum of a head is shared by the wave and moves only when a score exceeds it by more than 2^8 in the
-// weight (sums stay far inside fp32); then the sums are scaled. Sums, maxima and outputs are fp32. Rows outside the split
+// weight; then the sums are scaled. Sums, maxima and outputs are fp32, divided at the end: finite while the values' magnitude
+// times the number of keys is below 2^119 (2^8 in the weights, 2^127 in a sum). Rows outside the split
 // are never read: the loads go through buffer descriptors that end at the split's last key and give zeros behind it (codes
 // and scale: the value 0), and the weights of the last unit of keys are masked.
 #include "kvmx.h"
@@ -765,8 +770,12 @@ int launch(const char* what, const void* q, long ld_q, MXView kv, const int* kv_
     const int lds = loop > sums ? loop : sums;
     // More workgroups than the chip holds: behind the streams that start at once (their order does not matter, and it would
     // show as latency) the longest go first, or a long one that starts last runs on alone. 256 x 8 heads x 128, lengths up
-    // to 4096: 4 bits 106 us as numbered, 97 ordered; with 4 heads per kv head 124 and 110; lengths up to 2048 in 8 bits 118
-    // and 108; equal lengths 168 and 169. Short caches end before it pays (96 x 24 heads, 3 keys: 14.0 and 17.5).
+    // to 4096: 4 bits 103 us as numbered, 96 ordered, 8 bits 189 and 176; with 4 heads per kv head in 4 bits 115 and 105;
+    // lengths up to 2048 in 8 bits 99 and 100; equal lengths of 4096 321 and 325. Short caches end before it pays (96 x 24
+    // kv heads of 3 keys: one head each 7.0 and 10.1, four 16.6 and 19.9).
+    // MX_PLACES is a round figure for all instances: by registers and LDS they hold from 512 workgroups (several heads in 8
+    // bits, D = 128) to 1280 (one head), so where it is too high some streams that start late keep their place. With more than
+    // MX_ORDERED streams behind the first ones nothing is ordered.
     const long groups = (long)KVH * chunks * nsplit, at_once = MX_PLACES / groups;
     const int first = kv.max_len >= MX_ORDER_KEYS && B > at_once && B - at_once <= MX_ORDERED ? (int)at_once : B;
     if (lds > 65536) {                    // more than the default 64 KiB of dynamic LDS: asked for once per kernel and device
@@ -811,9 +820,10 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
     MGEN_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (D / 32 - 1)) == 0, "%s: scales must be aligned to a row (D / 32)", what);
     const MXView kv{(const unsigned char*)kc, (const unsigned char*)ks, (const unsigned char*)vc,
                     (const unsigned char*)vs, max_len};
-    // Several heads: 8 waves where a CU gets one workgroup or none (with loads to registers: 1 stream of 100003 keys, 4 kv heads
-    // of 4, 64 splits 25 us against 29 in workgroups of 4; 32 x 8 kv heads of 8, 4096 keys 48 and 54), 4 beyond (96 x 24, 3 keys:
-    // 27 and 14).
+    // Several heads: 8 waves where a CU gets one workgroup or none, 4 beyond. 8 and 4 waves, us: 32 x 8 kv heads of 4 x 128,
+    // 2000 keys in 4 bits 17.5 and 20.2, in 8 bits 27.6 and 27.8; 16 streams of 700 10.3 and 10.9; 1 of 100003 keys in 64 splits
+    // 25.4 and 25.1; 32 x 8 kv heads of 8, 4096 keys in 8 bits 49.9 and 47.9. Beyond: 40 streams of 1000 in 8 bits 24.1 and 21.1,
+    // 200 x 8 kv heads of 8, up to 2000 keys 97 and 77, 96 x 24 of 4, 3 keys 26.4 and 16.6.
 #define LAUNCH(DD, BB)                                                                                                 \
     do {                                                                                                               \
         if (H == KVH)                                                                                                  \
@@ -832,13 +842,17 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 
 // Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
 // Few workgroups: a power of two of splits (the chip's places divide evenly) that brings them to 512, to 1280 while each has
-// 1024 keys, and never less than two rounds of keys for a workgroup's waves; where the second launch is worth its 3 us, from
-// 8 rounds on. Measured, us: 1 stream x 8 heads x 128 in 8 bits, 4096 keys 33 in one split and 8.3 in 16, 512 keys 5.7 and
+// 1024 keys, but no more than leave a workgroup's waves two rounds of keys (that count as it is: 5 for one stream x 8 heads x
+// 128 of 1300 keys); where the second launch is worth its 3 us, from 8 rounds on. Measured, us: 1 stream x 8 heads x 128 in 8 bits, 4096 keys 33 in one split and 8.3 in 16, 512 keys 5.7 and
 // 7.6. 16 streams of 8 kv heads x 128 of up to 6000 keys, 4 heads each, 4 / 8 bits: 20.7 / 29.9 in 4 splits, 20.3 / 34.9 in
 // 6, 21.3 / 34.6 in 8; up to 32768 keys 79 / 119, 62 / 122, 59 / 116. 24 streams of up to 6000 keys, one head each, 26.5 / 38.7
 // in 2 splits, 19.8 / 33.7 in 4.
-// From 256 workgroups on: one (two, at 1500 keys: 1536 workgroups of heads of 64 in 4 bits 28 and 38 us, in 8 bits 50 and 52,
-// of 128 96 and 99; at 6000 keys 347 and 355).
+// From 256 workgroups on: one. One and two, at 1500 keys: 1536 workgroups of heads of 64 in 4 bits 28 and 38 us, in 8 bits 50
+// and 52, of 128 96 and 99; at 6000 keys 347 and 355. One and four at 256 workgroups, 32 streams x 8 kv heads x 128: all of
+// 16384 keys, 4 / 8 bits, 95 / 154 and 91 / 167, with 4 heads per kv head 93 / 167 and 100 / 172; all of 1500 14 / 20 and 15 / 22,
+// 16 / 23 and 20 / 30. The longest stream is all that the rule goes by, and where the others are shorter splits would pay at
+// such lengths: 1 to 16384 keys 94 / 147 and 59 / 110, with 4 heads 84 / 120 and 73 / 109; 1 to 4000 26 / 39 and 20 / 29, with 4
+// heads 27 / 34 and 26 / 38; 100 streams of 1 to 16384 160 / 332 and 130 / 236.
 extern "C" int mgen_attn_decode_mx_splits(int B, int H, int KVH, int D, int longest) {
     if (B <= 0 || KVH <= 0 || H < KVH || longest <= 0) return 1;
     const bool one = H == KVH;

@@ -1,6 +1,6 @@
 // The decode step's own token, taken from the raw projection rows inside an attention kernel: per-head RMSNorm and
 // rotation of one head row, shared by the attention over the bf16 cache (decode.hip) and over the quantised cache
-// (kvmx.hip), so that both work on the same keys and queries bit for bit.
+// (attn_decode_mx.hip), so that both work on the same keys and queries bit for bit.
 #pragma once
 #include "common.h"
 

@@ -4,7 +4,8 @@
 // Codes are e4m3 numbers (BITS = 8, largest 448, a byte each) or e2m1 numbers (BITS = 4, largest 6, the even element in
 // the low half of its byte). e is the smallest exponent at which the block's largest magnitude lies no further above the
 // largest code than half a step (464 = 448 + 16 and 7 = 6 + 1, ties to even), so that no element is rounded by more than
-// half a step of its own binade; it runs from 1 to the largest value at which every code is a finite float (246 / 252).
+// half a step of its own binade; it runs from 1 to the largest value at which every code is a finite float (246 / 252). (In 8
+// bits that ends at 448 * 2^119 = 2.98e38, and bf16 at 3.39e38: the elements between become the former.)
 // A block with an infinity or a NaN gets e = 255 and codes of zero and reads as NaN.
 // gfx950 converts two codes per instruction in both directions, exactly (scaled conversions round to nearest even and
 // saturate inside the range above), and every value is a bf16 number: the matrix instructions see the cache exactly.

@@ -6,7 +6,7 @@
 
 namespace {
 
-// n / d for n < 2^31 by a multiplication: q = (mulhi(n, m) + n) >> s
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, division by invariant integers): q = (mulhi(n, m) + n) >> s
 struct FastDiv {
     unsigned d, m, s;
 };

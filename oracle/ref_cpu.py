@@ -1,7 +1,7 @@
 """CPU oracle: a plain-torch restatement of the reference's decoder-only LM hot path.
 
 THIS IS TEST INFRASTRUCTURE. Only tests/, __graft_entry__.smoke() and the cpu_baseline leg of
-bench.py may import it. It is the checker, never the product: the product path lives in
+bench.py may import it. It is the oracle, never the product: the product path lives in
 symbolic-music-generation_amd/ and runs hand-written HIP kernels only.
 
 Every op is written out explicitly with torch CPU tensor arithmetic; nothing from `transformers`

@@ -2,7 +2,7 @@
 for a given mask.
 
 THIS IS TEST INFRASTRUCTURE. Only tests/, __graft_entry__.smoke() and the cpu_baseline leg of bench.py may import
-it. It is the checker, never the product.
+it. It is the oracle, never the product.
 
 What the reference does: GPT2LMHeadModel in training mode applies torch.nn.Dropout(0.1) to the summed embeddings
 (GPT2Model.forward, `self.drop`), to the attention probabilities after the softmax (eager_attention_forward /

@@ -1,7 +1,7 @@
 """CPU oracle for the reference's GPT-2 style decoder.
 
 THIS IS TEST INFRASTRUCTURE. Only tests/, __graft_entry__.smoke() and the cpu_baseline leg of bench.py may import
-it. It is the checker, never the product.
+it. It is the oracle, never the product.
 
 Plain-torch restatement, nothing imported from `transformers` or /root/reference. The reference builds
 transformers' GPT2LMHeadModel (/root/reference/src/model/model.py:54-65; transformers pinned 4.57.1 by its uv.lock);

@@ -1,7 +1,7 @@
 """CPU oracle for the reference's 4-D position model (notes as continuous [start, duration, pitch, velocity] rows).
 
 THIS IS TEST INFRASTRUCTURE. Only tests/, __graft_entry__.smoke() and the cpu_baseline leg of bench.py may import
-it. It is the checker, never the product.
+it. It is the oracle, never the product.
 
 Plain-torch restatement of the in-tree arithmetic of /root/reference, read as text; nothing is imported from it:
 

@@ -1,4 +1,4 @@
-"""Attention micro-benchmark on the GPU box (B=32, S=2048, H=8, D=128 by default), HIP-event timing per kernel."""
+"""Attention micro-benchmark on an MI355X (B=32, S=2048, H=8, D=128 by default), HIP-event timing per kernel."""
 import os, sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "symbolic-music-generation_amd"))

@@ -1,4 +1,4 @@
-"""Time the decode attention kernel alone (GPU box only): 256 streams x 8 heads x head_dim 128 (HEADS=H,KVH,D for another shape), bf16 K/V cache rows.
+"""Time the decode attention kernel alone (needs an MI355X): 256 streams x 8 heads x head_dim 128 (HEADS=H,KVH,D for another shape), bf16 K/V cache rows.
 Arguments: context length(s); MAXLEN=<n> sets the cache's row capacity (the pitch between streams)."""
 import os
 import sys

@@ -1,4 +1,4 @@
-"""Decode-only benchmark (GPU box): bench.py's two decode legs without the training step.
+"""Decode-only benchmark (MI355X): bench.py's two decode legs without the training step.
    python tools/bench_decode.py [repeats]      env: MGEN_DECODE_PARTS, MGEN_GEMM_SKINNY, LEGS=literal,long,short;
    MODEL=aria: the 650M Llama-style stand-in instead of the default decoder;
    KV=mxfp8 | mxfp4: that KV cache instead of bf16 (the fractions printed then count the bf16 cache's bytes);

@@ -1,4 +1,4 @@
-"""Time the HBM-bound kernels of one decoder layer at the training shape (GPU box only):
+"""Time the HBM-bound kernels of one decoder layer at the training shape (needs an MI355X):
 q/k-norm + RoPE forward and backward, RMSNorm backward, SwiGLU forward and backward."""
 import os
 import sys

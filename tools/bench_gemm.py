@@ -1,4 +1,4 @@
-"""GEMM micro-benchmark on the GPU box: the model's shapes through mgen_gemm_bf16, random data, HIP-event timing."""
+"""GEMM micro-benchmark on an MI355X: the model's shapes through mgen_gemm_bf16, random data, HIP-event timing."""
 import os, sys, time
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "symbolic-music-generation_amd"))

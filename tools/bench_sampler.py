@@ -1,4 +1,4 @@
-"""Time the next-token selection kernel on [B, V] bf16 logits (GPU box only)."""
+"""Time the next-token selection kernel on [B, V] bf16 logits (needs an MI355X)."""
 import os
 import sys
 import time

@@ -1,5 +1,5 @@
 // HBM streaming-rate probe: what a read+write element-wise kernel can reach on this chip, by access recipe.
-// Build: hipcc -O3 --offload-arch=gfx950 tools/lab/stream_rate.hip -o gpurun_out/stream_rate ; run on the GPU box.
+// Build: hipcc -O3 --offload-arch=gfx950 tools/lab/stream_rate.hip -o stream_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,6 +1,6 @@
 """Generate golden fixtures under tests/golden/ from the stock `transformers` modules the reference builds.
 
-Run ONLY in the build container (needs `transformers`; never runs on the GPU box, never imported by the
+Run ONLY in the build container (needs `transformers`; never runs beside a GPU, never imported by the
 product). The reference constructs its networks with AutoModelForCausalLM.from_config / GPT2LMHeadModel
 (/root/reference/src/model/model.py:65,136), i.e. the stock transformers classes; this script instantiates the
 same classes from explicit configs, runs them on seeded synthetic token batches and stores inputs + outputs.

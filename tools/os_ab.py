@@ -1,4 +1,4 @@
-"""Output-stationary weight-gradient GEMM against the tile-loop kernel on the GPU box (MGEN_GEMM_OS=0 switches the
+"""Output-stationary weight-gradient GEMM against the tile-loop kernel on an MI355X (MGEN_GEMM_OS=0 switches the
 new kernel off, read on every call): agreement up to the summation order, and timing."""
 import os, sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))

@@ -1,7 +1,8 @@
 #!/bin/bash
-# PMC passes over the attention micro-benchmark; results under gpurun_out/$1
+# PMC passes over the attention micro-benchmark; results under $OUT_DIR/$1 (profiles/raw by default)
 set -e
-OUT=$GRAFT_REPO_ROOT/gpurun_out/$1
+R=$(cd "$(dirname "$0")/.." && pwd)
+OUT=${OUT_DIR:-$R/profiles/raw}/$1
 mkdir -p $OUT
 cd /tmp && export TMPDIR=/tmp
 i=0
@@ -10,7 +11,7 @@ for C in "SQ_WAVE_CYCLES SQ_BUSY_CYCLES SQ_WAIT_ANY SQ_WAIT_INST_ANY SQ_ACTIVE_I
          "SQ_INST_CYCLES_VMEM SQ_ACTIVE_INST_MISC SQ_ACTIVE_INST_SCA SQ_INSTS_VALU_MFMA_MOPS_BF16 SQ_VALU_MFMA_COEXEC_CYCLES SQ_LDS_ADDR_CONFLICT SQ_LDS_UNALIGNED_STALL SQ_WAVES" \
          "GRBM_GUI_ACTIVE GRBM_COUNT"; do
   i=$((i+1))
-  timeout -s KILL 120 rocprofv3 --pmc $C --output-format csv -d $OUT/p$i -- python3 $GRAFT_REPO_ROOT/tools/bench_attn.py > $OUT/p$i.log 2>&1 || { tail -5 $OUT/p$i.log; exit 1; }
+  timeout -s KILL 120 rocprofv3 --pmc $C --output-format csv -d $OUT/p$i -- python3 $R/tools/bench_attn.py > $OUT/p$i.log 2>&1 || { tail -5 $OUT/p$i.log; exit 1; }
 done
-python3 $GRAFT_REPO_ROOT/tools/pmc_sum.py $OUT attn_ > $OUT/summary.txt
+python3 $R/tools/pmc_sum.py $OUT attn_ > $OUT/summary.txt
 cat $OUT/summary.txt

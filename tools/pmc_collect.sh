@@ -1,10 +1,10 @@
 #!/bin/bash
 # Counter and trace passes behind profiles/rNN_pmc_traffic.json and the kernel-stats files: `bash tools/pmc_collect.sh r02`
-# (on the GPU box; results under gpurun_out/<tag>/). One rocprofv3 run per counter, never combined with a trace.
+# (on an MI355X; results under $OUT_DIR/<tag>, profiles/raw by default). One rocprofv3 run per counter, never combined with a trace.
 set -e
 TAG=$1
-R=$GRAFT_REPO_ROOT
-OUT=$R/gpurun_out/$TAG
+R=$(cd "$(dirname "$0")/.." && pwd)
+OUT=${OUT_DIR:-$R/profiles/raw}/$TAG
 mkdir -p $OUT
 cd /tmp && export TMPDIR=/tmp
 TRAIN="$R/bench.py --steps 1 --warmup 1 --decode-tokens 0 --no-cpu-baseline"

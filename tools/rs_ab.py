@@ -1,4 +1,4 @@
-"""Register-panel GEMM (K = 512) against the tile-loop kernel on the GPU box: bit-for-bit equality and timing.
+"""Register-panel GEMM (K = 512) against the tile-loop kernel on an MI355X: bit-for-bit equality and timing.
 MGEN_GEMM_RS=0 (read on every call) switches the new kernel off."""
 import os, sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))

@@ -842,11 +842,12 @@ int attend(const char* what, const void* q, long ld_q, const void* kc, const voi
 
 // Key splits for a call whose longest stream has `longest` keys; never fewer for a longer one.
 // Few workgroups: a power of two of splits (the chip's places divide evenly) that brings them to 512, to 1280 while each has
-// 1024 keys, but no more than leave a workgroup's waves two rounds of keys (that count as it is: 5 for one stream x 8 heads x
-// 128 of 1300 keys); where the second launch is worth its 3 us, from 8 rounds on. Measured, us: 1 stream x 8 heads x 128 in 8 bits, 4096 keys 33 in one split and 8.3 in 16, 512 keys 5.7 and
-// 7.6. 16 streams of 8 kv heads x 128 of up to 6000 keys, 4 heads each, 4 / 8 bits: 20.7 / 29.9 in 4 splits, 20.3 / 34.9 in
-// 6, 21.3 / 34.6 in 8; up to 32768 keys 79 / 119, 62 / 122, 59 / 116. 24 streams of up to 6000 keys, one head each, 26.5 / 38.7
-// in 2 splits, 19.8 / 33.7 in 4.
+// 1024 keys, but no more than leave a workgroup's waves two rounds of keys (a limit that is no power of two: 5 for one
+// stream x 8 heads x 128 of 1300 keys); where the second launch is worth its 3 us, from 8 rounds on. Measured, us: 1 stream
+// x 8 heads x 128 in 8 bits, 4096 keys 33 in one split and 8.3 in 16, 512 keys 5.7 and 7.6. 16 streams of 8 kv heads x 128
+// of up to 6000 keys, 4 heads each, 4 / 8 bits: 20.7 / 29.9 in 4 splits, 20.3 / 34.9 in 6, 21.3 / 34.6 in 8; up to 32768
+// keys 79 / 119, 62 / 122, 59 / 116. 24 streams of up to 6000 keys, one head each, 26.5 / 38.7 in 2 splits, 19.8 / 33.7 in
+// 4.
 // From 256 workgroups on: one. One and two, at 1500 keys: 1536 workgroups of heads of 64 in 4 bits 28 and 38 us, in 8 bits 50
 // and 52, of 128 96 and 99; at 6000 keys 347 and 355. One and four at 256 workgroups, 32 streams x 8 kv heads x 128: all of
 // 16384 keys, 4 / 8 bits, 95 / 154 and 91 / 167, with 4 heads per kv head 93 / 167 and 100 / 172; all of 1500 14 / 20 and 15 / 22,
